@@ -126,9 +126,6 @@ def prepare(case, seed):
         strong = torch.bmm(normal(batch, c, rank) * torch.linspace(1.0, 0.1, rank, device="cuda"), normal(batch, rank, r))
         state["g"] = (1e-3 * (strong * rank ** -0.5 + 0.5 * normal(batch, c, r))).to(kind)
         state["out"] = torch.empty_like(state["g"])
-        if own:
-            import batchlas_b200 as bl
-            state["workspace"] = torch.empty(bl.newton_schulz_workspace_bytes(state["g"]), dtype=torch.uint8, device="cuda")
     return state
 
 
@@ -140,8 +137,7 @@ def _run_own(state):
     import batchlas_b200 as bl
     case = state["case"]
     if case["op"] == "newton_schulz":
-        return bl.newton_schulz(state["g"], state["out"], steps=case["steps"], coefficients=COEFFICIENTS, eps=EPS,
-                                workspace=state["workspace"])
+        return bl.newton_schulz(state["g"], state["out"], steps=case["steps"], coefficients=COEFFICIENTS, eps=EPS)
     bl.quantize_i8(state["x"], state["q"], state["scale"])
     if case["op"] == "quantize_i8":
         return {"values": state["q"] * state["scale"].unsqueeze(-1), "scale": state["scale"]}
