@@ -60,6 +60,34 @@ class EwiseDesc(ctypes.Structure):
                 ("dtype", ctypes.c_int32)]
 
 
+class QuantizeDesc(ctypes.Structure):
+    """Mirror of blb200_quantize_desc."""
+    _fields_ = [("x", ctypes.c_void_p), ("q", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("k", ctypes.c_int32), ("cols", ctypes.c_int32), ("batch", ctypes.c_int32),
+                ("ldx", ctypes.c_int64), ("stride_x", ctypes.c_int64), ("ldq", ctypes.c_int64),
+                ("stride_q", ctypes.c_int64), ("stride_scale", ctypes.c_int64), ("ftype", ctypes.c_int32)]
+
+
+class GemmI8Desc(ctypes.Structure):
+    """Mirror of blb200_gemm_i8_desc."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("c", ctypes.c_void_p),
+                ("scale_a", ctypes.c_void_p), ("scale_b", ctypes.c_void_p),
+                ("m", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("batch", ctypes.c_int32),
+                ("lda", ctypes.c_int64), ("ldb", ctypes.c_int64), ("ldc", ctypes.c_int64),
+                ("stride_a", ctypes.c_int64), ("stride_b", ctypes.c_int64), ("stride_c", ctypes.c_int64),
+                ("stride_scale_a", ctypes.c_int64), ("stride_scale_b", ctypes.c_int64),
+                ("alpha", ctypes.c_double), ("beta", ctypes.c_double), ("ftype_c", ctypes.c_int32)]
+
+
+class NewtonSchulzDesc(ctypes.Structure):
+    """Mirror of blb200_newton_schulz_desc."""
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p),
+                ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("batch", ctypes.c_int32),
+                ("ldx", ctypes.c_int64), ("ldy", ctypes.c_int64), ("stride_x", ctypes.c_int64), ("stride_y", ctypes.c_int64),
+                ("ftype", ctypes.c_int32), ("steps", ctypes.c_int32), ("coefficient_sets", ctypes.c_int32),
+                ("coefficients", ctypes.POINTER(ctypes.c_double)), ("eps", ctypes.c_double)]
+
+
 SIGNATURES = {
     "blb200_gemm_validate": (ctypes.c_int, [ctypes.POINTER(GemmDesc)]),
     "blb200_gemm_strided_batched": (ctypes.c_int, [ctypes.POINTER(GemmDesc), ctypes.c_void_p]),
@@ -107,6 +135,11 @@ SIGNATURES = {
     "blb200_arena_block_count": (ctypes.c_size_t, [ctypes.c_void_p]),
     "blb200_arena_alignment": (ctypes.c_size_t, [ctypes.c_void_p]),
     "blb200_measure_pipe_peak": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(ctypes.c_double)]),
+    "blb200_quantize_i8": (ctypes.c_int, [ctypes.POINTER(QuantizeDesc), ctypes.c_void_p]),
+    "blb200_gemm_i8": (ctypes.c_int, [ctypes.POINTER(GemmI8Desc), ctypes.c_void_p]),
+    "blb200_newton_schulz_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(NewtonSchulzDesc)]),
+    "blb200_newton_schulz": (ctypes.c_int, [ctypes.POINTER(NewtonSchulzDesc), ctypes.c_void_p, ctypes.c_size_t,
+                                            ctypes.c_void_p]),
     "blb200_fill": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint64, ctypes.c_uint64,
                                    ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int32, ctypes.c_double,
                                    ctypes.c_void_p]),

@@ -1,0 +1,193 @@
+// 8-bit integer products with scales:  C <- alpha diag(sa) A^T B diag(sb) + beta C,  A (k x m) and B (k x n)
+// int8 with k fastest.  The sums are exact 32-bit integers, so every kernel here gives the same bits.
+//
+// Tile kernel for any alignment: 128 x 128 of C per CTA, eight warps of 32 x 64, mma.sync m16n8k32 on
+// 64-byte k chunks staged in shared memory (pitch 80 bytes: the eight rows of a fragment request fall
+// into different banks).  Rows that start off a 4-byte boundary are read as aligned words and shifted
+// together; a word is read whole only where all of it lies inside the operand.
+#include "lowp.cuh"
+
+namespace blb200 {
+namespace {
+
+struct GemmI8Params {
+  const int8_t* a;
+  const int8_t* b;
+  void* c;
+  const float* scale_a;
+  const float* scale_b;
+  int m, n, k, batch;
+  long long lda, ldb, ldc, sa, sb, sc, ssa, ssb;
+  float alpha, beta;
+};
+
+// alpha * (acc * sa) * sb + beta * prior, in float, rounded once to T.
+template <typename T>
+__device__ __forceinline__ void store_c(T* c, int acc, float sa, float sb, float alpha, float beta) {
+  float v = alpha * (((float)acc * sa) * sb);
+  if (beta != 0.f) v = fmaf(beta, to_f32(*c), v);
+  *c = from_f32<T>(v);
+}
+
+constexpr int kTile = 128, kChunk = 64, kPitch = 80;
+
+// 16 bytes at `src` (any alignment) of which the first `valid` exist, the rest zero.  [lo, hi) is the operand.
+__device__ __forceinline__ uint4 load16_any(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (valid >= 16) {
+    const int off = (int)(reinterpret_cast<uintptr_t>(src) & 3u);
+    const int8_t* base = src - off;
+    if (off == 0) {
+      const uint32_t* s = reinterpret_cast<const uint32_t*>(base);
+      return make_uint4(s[0], s[1], s[2], s[3]);
+    }
+    if (base >= lo && base + 20 <= hi) {
+      const uint32_t* s = reinterpret_cast<const uint32_t*>(base);
+      const uint32_t x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3], x4 = s[4];
+      const int sh = off * 8;
+      return make_uint4(__funnelshift_r(x0, x1, sh), __funnelshift_r(x1, x2, sh), __funnelshift_r(x2, x3, sh),
+                        __funnelshift_r(x3, x4, sh));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < valid) w[i >> 2] |= (uint32_t)(uint8_t)src[i] << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void mma_i8(int (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) gemm_i8_any_kernel(GemmI8Params p, int tiles_m, long long tiles_per_item, long long tiles) {
+  __shared__ __align__(16) unsigned char tile_a[kTile * kPitch];
+  __shared__ __align__(16) unsigned char tile_b[kTile * kPitch];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int wm = (warp & 3) * 32, wn = (warp >> 2) * 64;
+  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const long long item = tile / tiles_per_item;
+    const int rem = (int)(tile - item * tiles_per_item);
+    const int m0 = rem % tiles_m * kTile, n0 = rem / tiles_m * kTile;
+    const int8_t* a = p.a + item * p.sa;
+    const int8_t* b = p.b + item * p.sb;
+    const int8_t* a_end = a + (long long)(p.m - 1) * p.lda + p.k;
+    const int8_t* b_end = b + (long long)(p.n - 1) * p.ldb + p.k;
+    int acc[2][8][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0;
+    uint4 next[4];
+    auto fetch = [&](int k0) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = tid + (u & 1) * 256, row = c >> 2, kk = k0 + (c & 3) * 16;
+        const bool is_a = u < 2;
+        const int r = (is_a ? m0 : n0) + row;
+        const int valid = r < (is_a ? p.m : p.n) ? p.k - kk : 0;
+        next[u] = valid > 0 ? load16_any((is_a ? a + (long long)r * p.lda : b + (long long)r * p.ldb) + kk, valid,
+                                         is_a ? a : b, is_a ? a_end : b_end)
+                            : make_uint4(0, 0, 0, 0);
+      }
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < p.k; k0 += kChunk) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = tid + (u & 1) * 256;
+        *reinterpret_cast<uint4*>((u < 2 ? tile_a : tile_b) + (c >> 2) * kPitch + (c & 3) * 16) = next[u];
+      }
+      __syncthreads();
+      if (k0 + kChunk < p.k) fetch(k0 + kChunk);
+#pragma unroll
+      for (int ks = 0; ks < kChunk; ks += 32) {
+        uint32_t fa[2][4], fb[8][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const unsigned char* s = tile_a + (wm + i * 16 + g) * kPitch + ks + t * 4;
+          fa[i][0] = *reinterpret_cast<const uint32_t*>(s);
+          fa[i][1] = *reinterpret_cast<const uint32_t*>(s + 8 * kPitch);
+          fa[i][2] = *reinterpret_cast<const uint32_t*>(s + 16);
+          fa[i][3] = *reinterpret_cast<const uint32_t*>(s + 8 * kPitch + 16);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned char* s = tile_b + (wn + j * 8 + g) * kPitch + ks + t * 4;
+          fb[j][0] = *reinterpret_cast<const uint32_t*>(s);
+          fb[j][1] = *reinterpret_cast<const uint32_t*>(s + 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mma_i8(acc[i][j], fa[i], fb[j]);
+      }
+      __syncthreads();
+    }
+    T* c = (T*)p.c + item * p.sc;
+    const float* sa = p.scale_a ? p.scale_a + item * p.ssa : nullptr;
+    const float* sb = p.scale_b ? p.scale_b + item * p.ssb : nullptr;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = m0 + wm + i * 16 + h * 8 + g;
+        if (row >= p.m) continue;
+        const float fsa = sa ? sa[row] : 1.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = n0 + wn + j * 8 + t * 2 + e;
+            if (col < p.n)
+              store_c(c + (long long)col * p.ldc + row, acc[i][j][h * 2 + e], fsa, sb ? sb[col] : 1.f, p.alpha, p.beta);
+          }
+      }
+  }
+}
+
+int launch_gemm_i8_any(const GemmI8Params& p, int ftype, cudaStream_t stream) {
+  const int tiles_m = (p.m + kTile - 1) / kTile;
+  const long long per_item = (long long)tiles_m * ((p.n + kTile - 1) / kTile), tiles = per_item * p.batch;
+  const long long cap = (long long)device_info().sm_count * 2;
+  return with_ftype(ftype, [&](auto t) {
+    gemm_i8_any_kernel<decltype(t)><<<(unsigned)(tiles < cap ? tiles : cap), 256, 0, stream>>>(p, tiles_m, per_item, tiles);
+    const int e = (int)cudaGetLastError();
+    if (e == 0) note_launch("gemm_i8_any");
+    return e;
+  });
+}
+
+constexpr int kMaxK = 131071;  // 128 * 128 * k stays below 2^31
+
+int validate_gemm_i8(const blb200_gemm_i8_desc* d) {
+  if (!d) return BLB200_E_NULL;
+  if (!valid_ftype(d->ftype_c)) return BLB200_E_DTYPE;
+  if (d->m < 0 || d->n < 0 || d->k < 0 || d->batch < 0) return BLB200_E_SHAPE;
+  if (d->k > kMaxK) return BLB200_E_TOO_LARGE;
+  if (!readable_layout(d->k, d->lda, d->stride_a) || !readable_layout(d->k, d->ldb, d->stride_b) ||
+      !writable_layout(d->m, d->n, d->batch, d->ldc, d->stride_c) || d->stride_scale_a < 0 || d->stride_scale_b < 0)
+    return BLB200_E_SHAPE;
+  if (d->m > 0 && d->n > 0 && d->batch > 0 && (!d->c || (d->k > 0 && (!d->a || !d->b)))) return BLB200_E_NULL;
+  return BLB200_OK;
+}
+
+}  // namespace
+}  // namespace blb200
+
+extern "C" int blb200_gemm_i8(const blb200_gemm_i8_desc* d, void* cuda_stream) {
+  using namespace blb200;
+  const int rc = validate_gemm_i8(d);
+  if (rc != BLB200_OK) return rc;
+  if (d->m == 0 || d->n == 0 || d->batch == 0) return BLB200_OK;
+  GemmI8Params p{d->a,   d->b,   d->c,        d->scale_a,  d->scale_b,  d->m,           d->n,
+                 d->k,   d->batch, d->lda,    d->ldb,      d->ldc,      d->stride_a,    d->stride_b,
+                 d->stride_c, d->stride_scale_a, d->stride_scale_b, (float)d->alpha, (float)d->beta};
+  if (p.k == 0) p.scale_a = p.scale_b = nullptr;  // C <- beta * C, whatever the scales hold
+  return launch_gemm_i8_any(p, d->ftype_c, (cudaStream_t)cuda_stream);
+}

@@ -1,0 +1,68 @@
+"""Orthogonalisation of update matrices by Newton-Schulz products, over torch tensors (device memory and streams
+only).  Matrices use the convention of :mod:`batchlas_b200.gemm`; since the iteration commutes with transposition, a
+row-major matrix can be passed as it is."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ._lib import NewtonSchulzDesc, check, load
+from .gemm import _as3
+from .quantized import FTYPE_CODES, _ld, _same_device, _st
+
+QUINTIC = (3.4445, -4.7750, 2.0315)
+
+
+def _desc(X, Y, steps, coefficients, eps):
+    if X.dtype not in FTYPE_CODES or Y.dtype != X.dtype:
+        raise TypeError("newton_schulz: X and Y must share one of float32/float16/bfloat16")
+    X3, Y3 = _as3(X), _as3(Y)
+    if X3.shape != Y3.shape:
+        raise RuntimeError("NEWTON_SCHULZ: incompatible matrix dimensions")
+    sets = list(coefficients)
+    if len(sets) == 3 and all(isinstance(v, (int, float)) for v in sets):
+        sets = [sets]
+    if len(sets) not in (1, steps) or any(len(s) != 3 for s in sets):
+        raise ValueError("newton_schulz: coefficients are one triple (a, b, c), or one for each step")
+    flat = [float(v) for s in sets for v in s]
+    d = NewtonSchulzDesc()
+    d.x, d.y = X3.data_ptr(), Y3.data_ptr()
+    d.batch, d.cols, d.rows = X3.shape
+    d.ldx, d.ldy, d.stride_x, d.stride_y = _ld(X3), _ld(Y3), _st(X3), _st(Y3)
+    d.ftype = FTYPE_CODES[X.dtype]
+    d.steps, d.coefficient_sets, d.eps = int(steps), len(sets), float(eps)
+    d.coefficients = (ctypes.c_double * len(flat))(*flat)
+    return d
+
+
+def newton_schulz_workspace_bytes(X) -> int:
+    """Scratch bytes that :func:`newton_schulz` needs for a tensor of X's shape and type."""
+    return int(load().blb200_newton_schulz_workspace_bytes(_desc(X, X, 1, QUINTIC, 0.0)))
+
+
+def newton_schulz(X, Y=None, steps=5, coefficients=QUINTIC, eps=1e-7, *, workspace=None, stream=None):
+    """Y <- X / (||X||_F + eps), then `steps` times Y <- (a I + b Y Y^T + c (Y Y^T)^2) Y, for every batch item; returns Y.
+
+    Y is made when it is not given and may be X.  float32 keeps float accuracy throughout; float16 and bfloat16 hold
+    the intermediate matrices in float16 with a common scale (half a step of 2^-12 each) and round Y once.  The scratch
+    comes from torch's caching allocator unless `workspace` (a CUDA uint8 tensor, 256-byte aligned, of at least
+    :func:`newton_schulz_workspace_bytes` bytes) is given.  Asynchronous."""
+    if Y is None:
+        Y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+    _same_device("batchlas_b200.newton_schulz", X, Y)
+    d = _desc(X, Y, steps, coefficients, eps)
+    with torch.cuda.device(Y.device):
+        need = int(load().blb200_newton_schulz_workspace_bytes(d))
+        if stream is None:
+            run_on = torch.cuda.current_stream()
+        else:
+            run_on = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+        if workspace is None:
+            with torch.cuda.stream(run_on):  # the scratch belongs to the stream that uses it
+                workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=Y.device)
+        elif workspace.device != Y.device or workspace.dtype != torch.uint8 or workspace.numel() < need \
+                or not workspace.is_contiguous() or workspace.data_ptr() % 256:
+            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {Y.device}, 256-byte aligned")
+        check(load().blb200_newton_schulz(d, workspace.data_ptr(), workspace.numel(), run_on.cuda_stream))
+    return Y

@@ -320,6 +320,75 @@ typedef struct blb200_ewise_desc {
 int blb200_elementwise(const blb200_ewise_desc* desc, int32_t op, void* cuda_stream);
 int blb200_axpby(const blb200_ewise_desc* desc, const double alpha[2], const double beta[2], void* cuda_stream);
 
+/* ---- products in the types of language models' layers ---------------------------------------
+ * 8-bit integer products with a scale for each token and channel, the quantiser that makes their
+ * operands, and the orthogonalisation of update matrices by Newton-Schulz products.  (BatchLAS has
+ * no counterpart: its scalars are float, double and their complex forms.)  Same conventions as
+ * above: column-major storage, leading dimensions and batch strides in elements, device pointers,
+ * asynchronous on `cuda_stream`, nothing allocated, status codes returned. */
+
+/* Floating storage type of an operand of these calls. */
+typedef enum { BLB200_F32 = 0, BLB200_F16 = 1, BLB200_BF16 = 2 } blb200_ftype;
+
+/* Quantises every column of a batch of k x cols matrices:
+ *     scale_j = fl32(max_i |x_ij| / 127),   q_ij = min(127, max(-127, rne(fl32(x_ij / scale_j))))
+ * with fl32 the rounding to float and rne the nearest integer, halves to the even one.  A column
+ * whose scale is 0 gets zeros (so an empty or all-zero column is exact); a column that holds a NaN or
+ * an infinity gets that as its scale, and zeros, so a product made with it is NaN there.
+ * scale: float, element j of item b at scale[b*stride_scale + j].  x, q and scale must not overlap.
+ * Padding rows (>= k within ldq) are not written. */
+typedef struct blb200_quantize_desc {
+  const void* x;
+  int8_t* q;
+  float* scale;
+  int32_t k, cols, batch;
+  int64_t ldx, stride_x, ldq, stride_q, stride_scale; /* elements */
+  int32_t ftype;                                      /* blb200_ftype of x */
+} blb200_quantize_desc;
+int blb200_quantize_i8(const blb200_quantize_desc* desc, void* cuda_stream);
+
+/* C_b <- alpha * diag(scale_a_b) * A_b^T * B_b * diag(scale_b_b) + beta * C_b, with A (k x m) and B (k x n) int8,
+ * both stored with k fastest (the T, N pair of gemm: one column per channel, one per token), C (m x n) in
+ * `ftype_c`.  The sums over k are exact 32-bit integers, hence k <= 131071, else BLB200_E_TOO_LARGE; the scales,
+ * alpha and beta are applied in float, and C is rounded once.  A null scale pointer stands for ones.
+ * stride_a, stride_b and the scales' strides may be 0 (one operand for the whole batch).
+ * m == 0 or n == 0 is a no-op, k == 0 scales C by beta, beta == 0 never reads C.  Operands whose base, ld and stride
+ * are multiples of 16 bytes take the tensor-map kernels, others the same sums at a lower rate. */
+typedef struct blb200_gemm_i8_desc {
+  const int8_t* a;
+  const int8_t* b;
+  void* c;
+  const float* scale_a; /* m per item, or null */
+  const float* scale_b; /* n per item, or null */
+  int32_t m, n, k, batch;
+  int64_t lda, ldb, ldc, stride_a, stride_b, stride_c;
+  int64_t stride_scale_a, stride_scale_b;
+  double alpha, beta;
+  int32_t ftype_c;
+} blb200_gemm_i8_desc;
+int blb200_gemm_i8(const blb200_gemm_i8_desc* desc, void* cuda_stream);
+
+/* Orthogonalises every matrix of a batch by `steps` Newton-Schulz products:
+ *     X <- G / (||G||_F + eps);   steps times:  S = X X^T,  X <- (a I + b S + c S^2) X      (rows <= cols;
+ * X^T X from the right otherwise), and writes the last X to y (y may be x itself, same ld and stride).
+ * coefficients: (a, b, c) once (coefficient_sets 1) or one triple per step (coefficient_sets == steps).
+ * From the coefficients follows a bound on X's largest singular value at each step; coefficients under
+ * which it passes 64, or an entry of b S + c S^2 may pass 16384, are refused with BLB200_E_TOO_LARGE.
+ * steps 1 .. 64, eps >= 0.  An item that holds a NaN or an infinity comes out as NaN.
+ * workspace: device memory of at least blb200_newton_schulz_workspace_bytes, 256-byte aligned. */
+typedef struct blb200_newton_schulz_desc {
+  const void* x;
+  void* y;
+  int32_t rows, cols, batch;
+  int64_t ldx, ldy, stride_x, stride_y; /* elements */
+  int32_t ftype;                        /* blb200_ftype of x and y */
+  int32_t steps, coefficient_sets;
+  const double* coefficients;           /* host memory */
+  double eps;
+} blb200_newton_schulz_desc;
+size_t blb200_newton_schulz_workspace_bytes(const blb200_newton_schulz_desc* desc);
+int blb200_newton_schulz(const blb200_newton_schulz_desc* desc, void* workspace, size_t workspace_bytes, void* cuda_stream);
+
 /* ---- synthetic inputs ------------------------------------------------------------------
  * Counter-based generator: element `i` of tensor `tensor_id` under `seed` depends only on
  * (seed, tensor_id, first_index + i), so any shard on any GPU count reproduces the same data.
