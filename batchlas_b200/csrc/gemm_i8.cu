@@ -6,6 +6,7 @@
 // into different banks).  Rows that start off a 4-byte boundary are read as aligned words and shifted
 // together; a word is read whole only where all of it lies inside the operand.
 #include "lowp.cuh"
+#include "umma_gemm.cuh"
 
 namespace blb200 {
 namespace {
@@ -163,6 +164,74 @@ int launch_gemm_i8_any(const GemmI8Params& p, int ftype, cudaStream_t stream) {
   });
 }
 
+// ---- tcgen05 tiles ---------------------------------------------------------------------------------
+// Rows of C (channels) on the M side, columns (tokens) on the N side: both operands are stored with k fastest, which
+// is the K-major form, and a thread of the epilogue owns one row, so that a warp stores 32 consecutive elements of a
+// column of C.
+enum { kUmmaI8Wait = 500 };
+
+template <typename T>
+struct I8Epilogue {
+  using Params = GemmI8Params;
+  T* c;
+  const float* sb;
+  const Params& p;
+  float sa;
+  bool live;
+  __device__ I8Epilogue(const Params& p_, const UmmaShape&, const UmmaTile& tile, int m) : p(p_), live(m < p_.m) {
+    c = (T*)p.c + (long long)tile.item * p.sc + m;
+    sa = p.scale_a && live ? p.scale_a[(long long)tile.item * p.ssa + m] : 1.f;
+    sb = p.scale_b ? p.scale_b + (long long)tile.item * p.ssb : nullptr;
+  }
+  template <int N>
+  __device__ void store(const uint32_t (&v)[N], int n) {
+    if (!live) return;
+    T* at = c + (long long)n * p.ldc;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (n + i < p.n) store_c(at + (long long)i * p.ldc, (int)v[i], sa, sb ? __ldg(sb + n + i) : 1.f, p.alpha, p.beta);
+  }
+};
+
+bool umma_i8_supported(const GemmI8Params& p) {
+  auto ok = [&](const int8_t* base, long long ld, long long stride, int cols) {
+    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (ld % 16 == 0 || cols == 1) && (stride % 16 == 0 || p.batch == 1);
+  };
+  return p.k > 0 && ok(p.a, p.lda, p.sa, p.m) && ok(p.b, p.ldb, p.sb, p.n) && encode_tiled_fn() != nullptr;
+}
+
+template <int GROUP, int BN>
+int launch_umma_i8(const GemmI8Params& p, int ftype, cudaStream_t stream) {
+  using C = UmmaConfig<true, false, false, GROUP, BN, 1>;
+  UmmaShape s{};
+  s.m = p.m;
+  s.n = p.n;
+  s.k = p.k;
+  s.batch = p.batch;
+  s.a_items = p.batch > 1 && p.sa == 0 ? 1 : p.batch;
+  s.b_items = p.batch > 1 && p.sb == 0 ? 1 : p.batch;
+  // a single column's ld is not used for addressing, but the map wants a multiple of 16
+  auto ld_of = [](long long ld, int cols) { return cols == 1 ? (ld + 15) / 16 * 16 : ld; };
+  CUtensorMap map_a, map_b;
+  int rc = encode_operand(&map_a, p.a, true, p.k, p.m, s.a_items, ld_of(p.lda, p.m), p.sa, 128);
+  if (rc == BLB200_OK) rc = encode_operand(&map_b, p.b, true, p.k, p.n, s.b_items, ld_of(p.ldb, p.n), p.sb, C::kBRows);
+  if (rc != BLB200_OK) return rc;
+  return with_ftype(ftype, [&](auto t) {
+    const int e = launch_umma<C, I8Epilogue<decltype(t)>>(map_a, map_b, s, p, kUmmaI8Wait, stream);
+    if (e == 0) note_launch("gemm_i8_umma");
+    return e;
+  });
+}
+
+int launch_umma_i8_any(const GemmI8Params& p, int ftype, cudaStream_t stream) {
+  if (p.n <= 16) return launch_umma_i8<1, 16>(p, ftype, stream);
+  if (p.n <= 32) return launch_umma_i8<1, 32>(p, ftype, stream);
+  if (p.n <= 64) return launch_umma_i8<1, 64>(p, ftype, stream);
+  const long long pairs = (long long)((p.m + 255) / 256) * ((p.n + 255) / 256) * p.batch, units = device_info().sm_count / 2;
+  if (pairs >= units) return launch_umma_i8<2, 256>(p, ftype, stream);
+  return launch_umma_i8<1, 128>(p, ftype, stream);
+}
+
 constexpr int kMaxK = 131071;  // 128 * 128 * k stays below 2^31
 
 int validate_gemm_i8(const blb200_gemm_i8_desc* d) {
@@ -178,6 +247,8 @@ int validate_gemm_i8(const blb200_gemm_i8_desc* d) {
 }
 
 }  // namespace
+int gemm_i8_device_status(int* out) { return read_device_status_word(out); }
+int gemm_i8_device_status_clear() { return clear_device_status_word(); }
 }  // namespace blb200
 
 extern "C" int blb200_gemm_i8(const blb200_gemm_i8_desc* d, void* cuda_stream) {
@@ -189,5 +260,9 @@ extern "C" int blb200_gemm_i8(const blb200_gemm_i8_desc* d, void* cuda_stream) {
                  d->k,   d->batch, d->lda,    d->ldb,      d->ldc,      d->stride_a,    d->stride_b,
                  d->stride_c, d->stride_scale_a, d->stride_scale_b, (float)d->alpha, (float)d->beta};
   if (p.k == 0) p.scale_a = p.scale_b = nullptr;  // C <- beta * C, whatever the scales hold
+  if (umma_i8_supported(p)) {
+    const int e = launch_umma_i8_any(p, d->ftype_c, (cudaStream_t)cuda_stream);
+    if (e != BLB200_E_INTERNAL) return e;  // a driver that refuses the tensor map: the tile kernel takes it
+  }
   return launch_gemm_i8_any(p, d->ftype_c, (cudaStream_t)cuda_stream);
 }

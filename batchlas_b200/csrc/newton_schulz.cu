@@ -4,6 +4,7 @@
 #include <math.h>
 
 #include "lowp.cuh"
+#include "ptx.cuh"
 
 namespace blb200 {
 namespace {
@@ -120,6 +121,8 @@ Layout layout_of(const blb200_newton_schulz_desc* d) {
 }
 
 }  // namespace
+int newton_schulz_device_status(int* out) { return read_device_status_word(out); }
+int newton_schulz_device_status_clear() { return clear_device_status_word(); }
 }  // namespace blb200
 
 extern "C" size_t blb200_newton_schulz_workspace_bytes(const blb200_newton_schulz_desc* d) {

@@ -11,6 +11,10 @@ int dmma_tma_device_status(int* out);
 int dmma_tma_device_status_clear();
 int sgemm_tma_device_status(int* out);
 int sgemm_tma_device_status_clear();
+int gemm_i8_device_status(int* out);
+int gemm_i8_device_status_clear();
+int newton_schulz_device_status(int* out);
+int newton_schulz_device_status_clear();
 int small_device_status_clear();
 int gemv_ring_device_status_clear();
 int small_ring_device_status_clear();
@@ -58,6 +62,14 @@ extern "C" int blb200_device_status(int* out) {
   }
   if (word == 0) {
     rc = blb200::sgemm_tma_device_status(&word);
+    if (rc != 0) return rc;
+  }
+  if (word == 0) {
+    rc = blb200::gemm_i8_device_status(&word);
+    if (rc != 0) return rc;
+  }
+  if (word == 0) {
+    rc = blb200::newton_schulz_device_status(&word);
     if (rc != 0) return rc;
   }
   if (word == 0) {

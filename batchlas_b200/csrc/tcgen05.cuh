@@ -1,0 +1,136 @@
+// Thin inline-PTX wrappers for the 5th-generation tensor cores of sm_100a: tensor memory, shared-memory and
+// instruction descriptors, MMA issue and commit, and the cluster forms of the mbarrier operations that a CTA pair
+// needs.  Waits are bounded as in ptx.cuh.
+#pragma once
+
+#include "tensor_map.cuh"
+
+namespace blb200 {
+
+// ---- clusters ------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of the same shared-memory location in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t smem, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int code) {
+  for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (spin > 64) __nanosleep(64);
+  }
+  atomicCAS(&g_device_status, 0, code);
+  return false;
+}
+// One box of a 3-D map into this CTA's shared memory, completion signalled on `bar`, a shared::cluster address that
+// may belong to the other CTA of the pair.  No multicast.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+// ---- tensor memory -------------------------------------------------------------------------------
+template <int GROUP>
+__device__ __forceinline__ void tmem_alloc(uint32_t* out_smem, uint32_t columns) {
+  if constexpr (GROUP == 1)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(out_smem)), "r"(columns) : "memory");
+  else
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(out_smem)), "r"(columns) : "memory");
+}
+template <int GROUP>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+  if constexpr (GROUP == 1) {
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+  } else {
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+  }
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Columns [addr, addr + 32 or 16) of the 32 lanes that belong to this warp's quarter of tensor memory.
+__device__ __forceinline__ void tmem_ld(uint32_t (&r)[32], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t (&r)[16], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+
+// ---- descriptors ---------------------------------------------------------------------------------
+// Shared-memory operand in the 128-byte swizzle.
+//   K-major:  128-byte rows (one per M or N index), groups of eight rows `stride_bytes` = 1024 apart; the k-step inside
+//             a row is taken by moving the start address.
+//   MN-major: 128-byte rows (one per k) of 64 half-precision M or N indices; groups of eight k rows 1024 bytes apart,
+//             blocks of 64 indices `lead_bytes` apart.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t smem, uint32_t lead_bytes, uint32_t stride_bytes) {
+  return (uint64_t)((smem & 0x3ffffu) >> 4) | ((uint64_t)(lead_bytes >> 4) << 16) | ((uint64_t)(stride_bytes >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor: s8 x s8 -> s32 or f16 x f16 -> f32, with each operand K-major or MN-major.
+__host__ __device__ constexpr uint32_t umma_idesc(bool i8, bool a_mn, bool b_mn, int m, int n) {
+  return ((i8 ? 2u : 1u) << 4) | ((i8 ? 1u : 0u) << 7) | ((i8 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// ---- MMA -----------------------------------------------------------------------------------------
+template <int GROUP, bool I8>
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  const uint32_t acc = accumulate ? 1u : 0u;
+#define BLB_UMMA(G, KIND)                                                                                          \
+  asm volatile(                                                                                                    \
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                                            \
+      "tcgen05.mma.cta_group::" #G ".kind::" #KIND " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) \
+      : "memory")
+  if constexpr (GROUP == 1 && I8) BLB_UMMA(1, i8);
+  else if constexpr (GROUP == 1) BLB_UMMA(1, f16);
+  else if constexpr (I8) BLB_UMMA(2, i8);
+  else BLB_UMMA(2, f16);
+#undef BLB_UMMA
+}
+// Arrives on `bar` (for a pair: on the barrier at this offset in both CTAs) when every MMA issued so far by this thread is done.
+template <int GROUP>
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  if constexpr (GROUP == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+
+}  // namespace blb200

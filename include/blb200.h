@@ -189,7 +189,8 @@ const char* blb200_version(void);
 int blb200_trace_flush(void);
 /* Synchronises the current device and reports whether any kernel of this library ever gave up
  * on one of its bounded waits: *out = 0 when none did, else a small code naming the wait
- * (1xx: 32^3 / 64^3 float rings, 2xx: gemv ring, 3xx: small-matrix ring, 4xx: TMA-fed DMMA tiles,
+ * (1xx: 32^3 / 64^3 float rings, 2xx: gemv ring, 3xx: small-matrix ring, 4xx: TMA-fed DMMA tiles, 5xx: 8-bit products,
+ * 6xx: Newton-Schulz products,
  * BLB200_WAIT_SELFTEST: the
  * self-test below).  Failure detection in the sense of BatchLAS's queue error handling
  * (src/util/queue-impl.cc wait_and_throw): the host learns of a lost copy instead of hanging. */
