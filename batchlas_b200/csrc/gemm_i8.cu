@@ -178,7 +178,7 @@ struct I8Epilogue {
   const Params& p;
   float sa;
   bool live;
-  __device__ I8Epilogue(const Params& p_, const UmmaShape&, const UmmaTile& tile, int m) : p(p_), live(m < p_.m) {
+  __device__ I8Epilogue(const Params& p_, const UmmaShape&, const UmmaTile& tile, bool, int m) : p(p_), live(m < p_.m) {
     c = (T*)p.c + (long long)tile.item * p.sc + m;
     sa = p.scale_a && live ? p.scale_a[(long long)tile.item * p.ssa + m] : 1.f;
     sb = p.scale_b ? p.scale_b + (long long)tile.item * p.ssb : nullptr;

@@ -11,7 +11,10 @@
 // Operands with K fastest are fetched as rows of 128 bytes (128 int8 or 64 half values of one M or N index); those with M or
 // N fastest (half only) as blocks of 64 indices x 64 k.  Both lie in the 128-byte swizzle.  Edges are zero-filled by
 // the map.  PLANES == 2: each operand is a pair hi + lo of half matrices (consecutive z slices of the map), and
-// hi*hi + hi*lo + lo*hi is accumulated: a float product but for the lo*lo term (2^-24 of the product).
+// hi*hi + hi*lo + lo*hi is accumulated: a float product but for the lo*lo term (2^-24 of the product).  The tensor
+// cores drop the bits below the accumulator's last one at every addition, which over a long k is a bias (k = 1501,
+// three products: 9.5e-6 of the iteration's result against 3e-6 for plain float sums); so for pairs only two k blocks (24
+// additions) are summed there, and the partial sums are added up in registers, rounded to nearest.
 //
 // A wait that runs out records its code, and the role leaves its loop; the other roles' waits then run out as well, the
 // copies still in flight are waited for, tensor memory is freed and the kernel returns.
@@ -38,12 +41,15 @@ struct UmmaConfig {
   static constexpr int GROUP = GROUP_, BN = BN_, PLANES = PLANES_;
   static constexpr int kBM = 128 * GROUP;              // rows of a tile
   static constexpr int kBRows = BN / GROUP;            // columns of B held by one CTA
+  static_assert(kBM == BN || kBM == 2 * BN || I8, "symmetric results need whole tiles on the diagonal");
   static constexpr int kKStage = I8 ? 128 : 64;        // k per stage: 128 bytes
   static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;
   static constexpr int kStageBytes = PLANES * (kABytes + kBBytes);
   static constexpr int kStages = (200 * 1024) / kStageBytes < 8 ? (200 * 1024) / kStageBytes : 8;
   static constexpr int kTmemColumns = 2 * BN < 32 ? 32 : 2 * BN;
   static constexpr int kThreads = 320;
+  static constexpr int kChunk = PLANES == 2 ? 2 : 0;   // k blocks summed in tensor memory, 0 = all
+  static constexpr int kRatio = kBM / BN;              // tile columns per tile row
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + 256;
   static_assert(!I8 || (!A_MN && !B_MN && PLANES == 1), "8-bit operands are K-major");
   static_assert(kStages >= 2 && kTmemColumns <= 512 && (kTmemColumns & (kTmemColumns - 1)) == 0, "");
@@ -53,18 +59,25 @@ struct UmmaTile {
   int item, tm, tn;
 };
 // Tiles of one item in an order that keeps the operands of the tiles in flight together in L2: bands of eight tile
-// rows, walked column by column; for a symmetric D the tiles on and below the diagonal, row by row.
+// rows, walked column by column; for a symmetric D the tiles that reach the diagonal or lie below it, row by row
+// (tile row i has R (i + 1) of them, R columns of tiles being as wide as one row of tiles is high).
+template <int R>
+__host__ __device__ inline long long symmetric_tiles(int tiles_m, int tiles_n) {
+  const long long full_rows = (long long)R * tiles_m * (tiles_m - 1) / 2, last = (long long)R * tiles_m;
+  return full_rows + (last < tiles_n ? last : tiles_n);
+}
+template <int R>
 __device__ __forceinline__ UmmaTile umma_tile(const UmmaShape& s, long long t) {
   UmmaTile r;
   if (s.symmetric) {
-    const long long per = (long long)s.tiles_m * (s.tiles_m + 1) / 2;
+    const long long per = symmetric_tiles<R>(s.tiles_m, s.tiles_n);
     r.item = (int)(t / per);
     const int f = (int)(t - (long long)r.item * per);
-    int i = (int)((sqrtf(8.f * (float)f + 1.f) - 1.f) * 0.5f);
-    while ((long long)(i + 1) * (i + 2) / 2 <= f) ++i;
-    while ((long long)i * (i + 1) / 2 > f) --i;
+    int i = (int)((sqrtf((8.f / R) * (float)f + 1.f) - 1.f) * 0.5f);
+    while ((long long)R * (i + 1) * (i + 2) / 2 <= f) ++i;
+    while ((long long)R * i * (i + 1) / 2 > f) --i;
     r.tm = i;
-    r.tn = f - (int)((long long)i * (i + 1) / 2);
+    r.tn = f - (int)((long long)R * i * (i + 1) / 2);
     return r;
   }
   const long long per = (long long)s.tiles_m * s.tiles_n;
@@ -126,7 +139,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       uint32_t round = 0;
       int slot = 0;
       for (long long t = first; t < s.tiles && ok; t += step) {
-        const UmmaTile tile = umma_tile(s, t);
+        const UmmaTile tile = umma_tile<C::kRatio>(s, t);
         const int za = (s.a_items == 1 ? 0 : tile.item) * C::PLANES, zb = (s.b_items == 1 ? 0 : tile.item) * C::PLANES;
         const int m0 = tile.tm * C::kBM + (int)rank * 128, n0 = tile.tn * C::BN + (int)rank * C::kBRows;
         for (int kb = 0; kb < k_blocks && ok; ++kb) {
@@ -193,14 +206,17 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       uint32_t round = 0;
       int slot = 0;
       long long done = 0;
-      for (long long t = first; t < s.tiles && ok; t += step, ++done) {
-        const int acc = (int)(done & 1);
-        ok = G == 1 ? mbar_wait(&acc_free[acc], (uint32_t)((done >> 1) & 1) ^ 1, wait_code + kUmmaWaitAccFree)
-                    : mbar_wait_cluster(&acc_free[acc], (uint32_t)((done >> 1) & 1) ^ 1, wait_code + kUmmaWaitAccFree);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t d = tmem + acc * C::BN;
+      for (long long t = first; t < s.tiles && ok; t += step) {
+        uint32_t d = 0;
         for (int kb = 0; kb < k_blocks; ++kb) {
+          const bool begins = C::kChunk ? kb % (C::kChunk ? C::kChunk : 1) == 0 : kb == 0;
+          if (begins) {
+            const int acc = (int)(done & 1);
+            ok = G == 1 ? mbar_wait(&acc_free[acc], (uint32_t)((done >> 1) & 1) ^ 1, wait_code + kUmmaWaitAccFree)
+                        : mbar_wait_cluster(&acc_free[acc], (uint32_t)((done >> 1) & 1) ^ 1, wait_code + kUmmaWaitAccFree);
+            if (!ok) break;
+            d = tmem + acc * C::BN;
+          }
           ok = G == 1 ? mbar_wait(&full[slot], round & 1, wait_code + kUmmaWaitFull)
                       : mbar_wait_cluster(&full[slot], round & 1, wait_code + kUmmaWaitFull);
           if (!ok) break;
@@ -212,7 +228,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             const uint64_t da = umma_desc(a + ks * kAStep, kALead, 1024), db = umma_desc(b + ks * kBStep, kBLead, 1024);
-            umma<G, C::I8>(d, da, db, idesc, kb > 0 || ks > 0);
+            umma<G, C::I8>(d, da, db, idesc, !begins || ks > 0);
             if constexpr (C::PLANES == 2) {
               const uint64_t da2 = umma_desc(a + C::kABytes + ks * kAStep, kALead, 1024);
               const uint64_t db2 = umma_desc(b + C::kBBytes + ks * kBStep, kBLead, 1024);
@@ -225,41 +241,76 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             slot = 0;
             ++round;
           }
+          if (kb + 1 == k_blocks || (C::kChunk && (kb + 1) % (C::kChunk ? C::kChunk : 1) == 0)) {
+            umma_commit<G>(&acc_full[done & 1]);
+            ++done;
+          }
         }
-        if (ok) umma_commit<G>(&acc_full[acc]);
       }
     }
   } else {
     // Two warps per quarter of the 128 rows: each takes half of the columns (narrow tiles: the first takes all).
-    constexpr int kSplit = C::BN >= 64 ? 2 : 1, kCols = C::BN / kSplit, kChunk = kCols < 32 ? 16 : 32;
+    constexpr int kSplit = C::BN >= 64 ? 2 : 1, kCols = C::BN / kSplit, kPiece = kCols < 32 ? 16 : 32;
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const int row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + half * kCols;
     long long done = 0;
-    for (long long t = first; t < s.tiles; t += step, ++done) {
-      const UmmaTile tile = umma_tile(s, t);
+    auto acquire = [&]() {
       const int acc = (int)(done & 1);
       const bool ok = G == 1 ? mbar_wait(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc)
                              : mbar_wait_cluster(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
-      const int m = tile.tm * C::kBM + (int)rank * 128 + row;
-      const int n0 = tile.tn * C::BN + half * kCols;
-      if (half < kSplit) {
-        Epilogue epi(ep, s, tile, m);
-#pragma unroll 1
-        for (int c = 0; c < kCols; c += kChunk) {
-          if (n0 + c >= s.n) break;
-          uint32_t v[kChunk];
-          tmem_ld(v, tmem + ((uint32_t)(quarter * 32) << 16) + acc * C::BN + half * kCols + c);
-          tmem_wait_ld();
-          epi.store(v, n0 + c);
-        }
-      }
+      return true;
+    };
+    auto release = [&]() {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (G == 2) mbar_arrive_cluster(cluster_addr(smem_u32(&acc_free[acc]), 0));
-        else mbar_arrive(&acc_free[acc]);
+        if constexpr (G == 2) mbar_arrive_cluster(cluster_addr(smem_u32(&acc_free[done & 1]), 0));
+        else mbar_arrive(&acc_free[done & 1]);
+      }
+      ++done;
+    };
+    bool ok = true;
+    for (long long t = first; t < s.tiles && ok; t += step) {
+      const UmmaTile tile = umma_tile<C::kRatio>(s, t);
+      const int n0 = tile.tn * C::BN + half * kCols;
+      Epilogue epi(ep, s, tile, s.symmetric && tile.tn < C::kRatio * tile.tm, tile.tm * C::kBM + (int)rank * 128 + row);
+      if constexpr (C::kChunk == 0) {
+        ok = acquire();
+        if (!ok) break;
+        if (half < kSplit) {
+#pragma unroll 1
+          for (int c = 0; c < kCols; c += kPiece) {
+            if (n0 + c >= s.n) break;
+            uint32_t v[kPiece];
+            tmem_ld(v, lanes + (uint32_t)(done & 1) * C::BN + c);
+            tmem_wait_ld();
+            epi.store(v, n0 + c);
+          }
+        }
+        release();
+      } else {
+        uint32_t v[kCols / kPiece][kPiece] = {};
+        for (int kb = 0; kb < k_blocks; kb += C::kChunk) {
+          ok = acquire();
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < kCols / kPiece; ++c) {
+            uint32_t w[kPiece];
+            tmem_ld(w, lanes + (uint32_t)(done & 1) * C::BN + c * kPiece);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < kPiece; ++i)
+              v[c][i] = __float_as_uint(__uint_as_float(v[c][i]) + __uint_as_float(w[i]));
+          }
+          release();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < kCols / kPiece; ++c)
+          if (n0 + c * kPiece < s.n) epi.store(v[c], n0 + c * kPiece);
       }
     }
   }
@@ -292,7 +343,7 @@ int launch_umma(const CUtensorMap& map_a, const CUtensorMap& map_b, UmmaShape s,
                 cudaStream_t stream) {
   s.tiles_m = (s.m + C::kBM - 1) / C::kBM;
   s.tiles_n = (s.n + C::BN - 1) / C::BN;
-  s.tiles = (s.symmetric ? (long long)s.tiles_m * (s.tiles_m + 1) / 2 : (long long)s.tiles_m * s.tiles_n) * s.batch;
+  s.tiles = (s.symmetric ? symmetric_tiles<C::kRatio>(s.tiles_m, s.tiles_n) : (long long)s.tiles_m * s.tiles_n) * s.batch;
   auto kern = umma_gemm_kernel<C, Epilogue>;
   static thread_local int configured_for = -1;
   int cur = 0;

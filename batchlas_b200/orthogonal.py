@@ -8,8 +8,7 @@ import ctypes
 import torch
 
 from ._lib import NewtonSchulzDesc, check, load
-from .gemm import _as3
-from .quantized import FTYPE_CODES, _ld, _same_device, _st
+from .quantized import FTYPE_CODES, _matrix, _same_device
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
 
@@ -17,8 +16,9 @@ QUINTIC = (3.4445, -4.7750, 2.0315)
 def _desc(X, Y, steps, coefficients, eps):
     if X.dtype not in FTYPE_CODES or Y.dtype != X.dtype:
         raise TypeError("newton_schulz: X and Y must share one of float32/float16/bfloat16")
-    X3, Y3 = _as3(X), _as3(Y)
-    if X3.shape != Y3.shape:
+    batch, cols, rows, ldx, stride_x = _matrix(X)
+    y_batch, y_cols, y_rows, ldy, stride_y = _matrix(Y)
+    if (batch, cols, rows) != (y_batch, y_cols, y_rows):
         raise RuntimeError("NEWTON_SCHULZ: incompatible matrix dimensions")
     sets = list(coefficients)
     if len(sets) == 3 and all(isinstance(v, (int, float)) for v in sets):
@@ -26,14 +26,8 @@ def _desc(X, Y, steps, coefficients, eps):
     if len(sets) not in (1, steps) or any(len(s) != 3 for s in sets):
         raise ValueError("newton_schulz: coefficients are one triple (a, b, c), or one for each step")
     flat = [float(v) for s in sets for v in s]
-    d = NewtonSchulzDesc()
-    d.x, d.y = X3.data_ptr(), Y3.data_ptr()
-    d.batch, d.cols, d.rows = X3.shape
-    d.ldx, d.ldy, d.stride_x, d.stride_y = _ld(X3), _ld(Y3), _st(X3), _st(Y3)
-    d.ftype = FTYPE_CODES[X.dtype]
-    d.steps, d.coefficient_sets, d.eps = int(steps), len(sets), float(eps)
-    d.coefficients = (ctypes.c_double * len(flat))(*flat)
-    return d
+    return NewtonSchulzDesc(X.data_ptr(), Y.data_ptr(), rows, cols, batch, ldx, ldy, stride_x, stride_y, FTYPE_CODES[X.dtype], int(steps),
+                            len(sets), (ctypes.c_double * len(flat))(*flat), float(eps))
 
 
 def newton_schulz_workspace_bytes(X) -> int:
@@ -44,8 +38,9 @@ def newton_schulz_workspace_bytes(X) -> int:
 def newton_schulz(X, Y=None, steps=5, coefficients=QUINTIC, eps=1e-7, *, workspace=None, stream=None):
     """Y <- X / (||X||_F + eps), then `steps` times Y <- (a I + b Y Y^T + c (Y Y^T)^2) Y, for every batch item; returns Y.
 
-    Y is made when it is not given and may be X.  float32 keeps float accuracy throughout; float16 and bfloat16 hold
-    the intermediate matrices in float16 with a common scale (half a step of 2^-12 each) and round Y once.  The scratch
+    Y is made when it is not given and may be X.  float32 and float16 keep float accuracy throughout (every
+    intermediate matrix is a pair of float16 matrices); bfloat16 keeps one float16 matrix of each, times a power of two.
+    Y is rounded once.  The scratch
     comes from torch's caching allocator unless `workspace` (a CUDA uint8 tensor, 256-byte aligned, of at least
     :func:`newton_schulz_workspace_bytes` bytes) is given.  Asynchronous."""
     if Y is None:

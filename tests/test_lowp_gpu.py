@@ -6,7 +6,7 @@ gemm_i8      the integer sums are exact; scale_a, scale_b, alpha and the convers
                  |C - exact| <= 4 u |alpha S sa sb| + (u + u_T) |exact| + the smallest subnormal of the type.
 newton_schulz  in the 2-norm (Frobenius) against 64 bits, by emulations in 64 bits that disturb every stored matrix (X, S, B of
              each step) by independent relative errors, uniform up to the size that one store makes: half a step of
-             float16 (2^-11) for the half types; for float 2^-22 per stored pair plus the float accumulation of a
+             float16 (2^-11) for bfloat16; for float and float16 2^-22 per stored pair plus the float accumulation of a
              k-long sum (k/16 additions of one half-step 2^-24 each, three products).  With r the root mean square of the
              emulations' errors the allowed error is sqrt(9 steps) r, and half a step for Y.  To first order the error is a sum
              of one term per stored matrix, 3 steps of them.  A store's true error is at most sqrt(3) times the uniform
@@ -262,7 +262,7 @@ def newton_schulz_reference(g, steps, sets, eps, disturb=0.0, seed=0):
 def newton_schulz_check(got, g, kind, steps=5, sets=(QUINTIC,), eps=1e-7):
     want = newton_schulz_reference(g, steps, sets, eps)
     p, q = sorted(g.shape[1:])
-    one_store = 2.0 ** -11 if kind != "f32" else 2.0 ** -22 + 3 * (q / 16 + 1) * 2.0 ** -24
+    one_store = 2.0 ** -11 if kind == "bf16" else 2.0 ** -22 + 3 * (q / 16 + 1) * 2.0 ** -24
     errors = torch.stack([newton_schulz_reference(g, steps, sets, eps, one_store, seed=p + q + i) - want for i in range(8)])
     rms = errors.square().sum((2, 3)).mean(0).sqrt()
     for i in range(g.shape[0]):
