@@ -5,6 +5,8 @@
 // 64-byte k chunks staged in shared memory (pitch 80 bytes: the eight rows of a fragment request fall
 // into different banks).  Rows that start off a 4-byte boundary are read as aligned words and shifted
 // together; a word is read whole only where all of it lies inside the operand.
+#include <type_traits>
+
 #include "lowp.cuh"
 #include "umma_gemm.cuh"
 
@@ -164,6 +166,138 @@ int launch_gemm_i8_any(const GemmI8Params& p, int ftype, cudaStream_t stream) {
   });
 }
 
+// ---- few columns -----------------------------------------------------------------------------------
+// Up to 32 tokens: the weights are read once and that is the time.  A CTA owns MT tiles of 16 rows of C; its eight warps
+// split k, and every lane holds its share of a 16 x 64 slab of weights by two 16-byte loads straight into mma.sync
+// fragments: the order of k inside a slab does not matter as long as both operands share it, so lane (g, t) takes bytes
+// 16 t .. 16 t + 15 of rows g and g + 8 (and of token g), words 0, 1 for one instruction and 2, 3 for the next.  The slabs of
+// kFlight row tiles and k steps are in flight per warp before the first is used.  The more rows a CTA owns, the less often
+// the tokens are read (from L2); the fewer, the more SMs take part.  Before it waits for the kernel that produced
+// its tokens, each lane asks for its first weights to be brought into L2, which has no effect but on time.  The warps' sums
+// meet in shared memory.
+constexpr int kFlight = 4;
+
+template <bool WHOLE>
+__device__ __forceinline__ uint4 load16(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
+  if (WHOLE && valid >= 16) return *reinterpret_cast<const uint4*>(src);
+  if (valid <= 0) return make_uint4(0, 0, 0, 0);
+  return load16_any(src, valid, lo, hi);
+}
+
+// WHOLE: both operands' columns start on 16-byte boundaries.
+template <typename T, int NT, int MT, bool WHOLE>
+__global__ void __launch_bounds__(256) gemm_i8_few_kernel(GemmI8Params p, int tiles_m) {
+  constexpr int kSlabs = kFlight / MT;  // k steps in flight
+  __shared__ int part[8][NT][16][9];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long item = blockIdx.x / tiles_m;
+  const int m0 = (int)(blockIdx.x - item * tiles_m) * 16 * MT;
+  const int8_t* a = p.a + item * p.sa;
+  const int8_t* b = p.b + item * p.sb;
+  const int8_t* a_end = a + (long long)(p.m - 1) * p.lda + p.k;
+  const int8_t* b_end = b + (long long)(p.n - 1) * p.ldb + p.k;
+  // this warp's k range, in whole slabs
+  const int slabs = (p.k + 63) / 64, each = (slabs + 7) / 8;
+  const int k_begin = warp * each * 64 + t * 16, k_end = min(p.k, (warp + 1) * each * 64);
+  const int8_t* row[2 * MT];
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) row[i] = a + (long long)min(m0 + g + 8 * i, p.m - 1) * p.lda;
+  const int8_t* col[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) col[j] = b + (long long)min(8 * j + g, p.n - 1) * p.ldb;
+#pragma unroll
+  for (int s = 0; s < kSlabs; ++s)
+    if (k_begin + 64 * s < k_end) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) asm volatile("prefetch.global.L2 [%0];" ::"l"(row[i] + k_begin + 64 * s));
+    }
+  griddep_wait();
+  griddep_launch();
+
+  int acc[MT][NT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0;
+  for (int k0 = k_begin; k0 - t * 16 < k_end; k0 += 64 * kSlabs) {
+    uint4 w[kSlabs][2 * MT], x[kSlabs][NT];
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) w[s][i] = load16<WHOLE>(row[i] + k0 + 64 * s, k_end - (k0 + 64 * s), a, a_end);
+    }
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) x[s][j] = load16<WHOLE>(col[j] + k0 + 64 * s, k_end - (k0 + 64 * s), b, b_end);
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const uint4 lo = w[s][2 * i], hi = w[s][2 * i + 1], y = x[s][j];
+          const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, b0[2] = {y.x, y.y};
+          const uint32_t a1[4] = {lo.z, hi.z, lo.w, hi.w}, b1[2] = {y.z, y.w};
+          mma_i8(acc[i][j], a0, b0);
+          mma_i8(acc[i][j], a1, b1);
+        }
+  }
+  T* c = (T*)p.c + item * p.sc;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    if (i > 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[warp][j][g + 8 * (e >> 1)][2 * t + (e & 1)] = acc[i][j][e];
+    __syncthreads();
+    for (int o = threadIdx.x; o < 16 * 8 * NT; o += 256) {
+      const int r = o & 15, n = o >> 4, m = m0 + 16 * i + r;
+      if (m >= p.m || n >= p.n) continue;
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) sum += part[w][n >> 3][r][n & 7];
+      store_c(c + (long long)n * p.ldc + m, sum, p.scale_a ? p.scale_a[item * p.ssa + m] : 1.f,
+              p.scale_b ? p.scale_b[item * p.ssb + n] : 1.f, p.alpha, p.beta);
+    }
+  }
+}
+
+bool columns_16(const int8_t* base, long long ld, long long stride, int cols, int batch) {
+  return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (ld % 16 == 0 || cols == 1) && (stride % 16 == 0 || batch == 1);
+}
+
+int launch_gemm_i8_few(const GemmI8Params& p, int ftype, cudaStream_t stream) {
+  const bool whole = columns_16(p.a, p.lda, p.sa, p.m, p.batch) && columns_16(p.b, p.ldb, p.sb, p.n, p.batch);
+  // as many rows per CTA as leave a CTA for every SM
+  const long long sms = device_info().sm_count;
+  auto ctas = [&](int mt) { return (long long)((p.m + 16 * mt - 1) / (16 * mt)) * p.batch; };
+  const int mt = ctas(4) >= sms ? 4 : ctas(2) >= sms ? 2 : 1;
+  const OverlappedLaunch launch((unsigned)ctas(mt), 256, stream);
+  const int tiles_m = (p.m + 16 * mt - 1) / (16 * mt);
+  return with_ftype(ftype, [&](auto v) {
+    using T = decltype(v);
+    auto with_rows = [&](auto nt, auto rows) {
+      constexpr int NT = decltype(nt)::value, MT = decltype(rows)::value;
+      return whole ? cudaLaunchKernelEx(&launch.cfg, gemm_i8_few_kernel<T, NT, MT, true>, p, tiles_m)
+                   : cudaLaunchKernelEx(&launch.cfg, gemm_i8_few_kernel<T, NT, MT, false>, p, tiles_m);
+    };
+    auto with_columns = [&](auto nt) {
+      return mt == 4   ? with_rows(nt, std::integral_constant<int, 4>{})
+             : mt == 2 ? with_rows(nt, std::integral_constant<int, 2>{})
+                       : with_rows(nt, std::integral_constant<int, 1>{});
+    };
+    const cudaError_t e = p.n <= 8    ? with_columns(std::integral_constant<int, 1>{})
+                          : p.n <= 16 ? with_columns(std::integral_constant<int, 2>{})
+                                      : with_columns(std::integral_constant<int, 4>{});
+    if (e == cudaSuccess) note_launch("gemm_i8_few");
+    return (int)e;
+  });
+}
+
 // ---- tcgen05 tiles ---------------------------------------------------------------------------------
 // Rows of C (channels) on the M side, columns (tokens) on the N side: both operands are stored with k fastest, which
 // is the K-major form, and a thread of the epilogue owns one row, so that a warp stores 32 consecutive elements of a
@@ -189,15 +323,12 @@ struct I8Epilogue {
     T* at = c + (long long)n * p.ldc;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (n + i < p.n) store_c(at + (long long)i * p.ldc, (int)v[i], sa, sb ? __ldg(sb + n + i) : 1.f, p.alpha, p.beta);
+      if (n + i < p.n) store_c(at + (long long)i * p.ldc, (int)v[i], sa, sb ? sb[n + i] : 1.f, p.alpha, p.beta);
   }
 };
 
 bool umma_i8_supported(const GemmI8Params& p) {
-  auto ok = [&](const int8_t* base, long long ld, long long stride, int cols) {
-    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (ld % 16 == 0 || cols == 1) && (stride % 16 == 0 || p.batch == 1);
-  };
-  return p.k > 0 && ok(p.a, p.lda, p.sa, p.m) && ok(p.b, p.ldb, p.sb, p.n) && encode_tiled_fn() != nullptr;
+  return p.k > 0 && columns_16(p.a, p.lda, p.sa, p.m, p.batch) && columns_16(p.b, p.ldb, p.sb, p.n, p.batch) && encode_tiled_fn() != nullptr;
 }
 
 template <int GROUP, int BN>
@@ -224,8 +355,6 @@ int launch_umma_i8(const GemmI8Params& p, int ftype, cudaStream_t stream) {
 }
 
 int launch_umma_i8_any(const GemmI8Params& p, int ftype, cudaStream_t stream) {
-  if (p.n <= 16) return launch_umma_i8<1, 16>(p, ftype, stream);
-  if (p.n <= 32) return launch_umma_i8<1, 32>(p, ftype, stream);
   if (p.n <= 64) return launch_umma_i8<1, 64>(p, ftype, stream);
   const long long pairs = (long long)((p.m + 255) / 256) * ((p.n + 255) / 256) * p.batch, units = device_info().sm_count / 2;
   if (pairs >= units) return launch_umma_i8<2, 256>(p, ftype, stream);
@@ -260,6 +389,8 @@ extern "C" int blb200_gemm_i8(const blb200_gemm_i8_desc* d, void* cuda_stream) {
                  d->k,   d->batch, d->lda,    d->ldb,      d->ldc,      d->stride_a,    d->stride_b,
                  d->stride_c, d->stride_scale_a, d->stride_scale_b, (float)d->alpha, (float)d->beta};
   if (p.k == 0) p.scale_a = p.scale_b = nullptr;  // C <- beta * C, whatever the scales hold
+  if (p.n <= 32 && p.k > 0 && ((long long)(p.m + 15) / 16) * p.batch <= 0x7fffffffll)
+    return launch_gemm_i8_few(p, d->ftype_c, (cudaStream_t)cuda_stream);
   if (umma_i8_supported(p)) {
     const int e = launch_umma_i8_any(p, d->ftype_c, (cudaStream_t)cuda_stream);
     if (e != BLB200_E_INTERNAL) return e;  // a driver that refuses the tensor map: the tile kernel takes it

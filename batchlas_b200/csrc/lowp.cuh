@@ -44,4 +44,23 @@ inline bool writable_layout(long long rows, long long cols, long long batch, lon
   return stride >= (cols - 1) * ld + rows || (stride >= rows && ld >= (batch - 1) * stride + rows);
 }
 
+// Launch configuration that lets a kernel's start overlap the end of the kernel before it in the stream.  Such a kernel
+// calls griddep_wait() before it touches global memory; griddep_launch() lets its own successor start likewise.
+struct OverlappedLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  OverlappedLaunch(dim3 grid, dim3 block, cudaStream_t stream) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  OverlappedLaunch(const OverlappedLaunch&) = delete;
+};
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 }  // namespace blb200

@@ -78,6 +78,8 @@ struct Unit {
 // Sum of squares in double (float's whole range, squared, fits), one part per block, in a fixed order.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) norm_parts_kernel(Matrices g, double* parts, int tx) {
+  griddep_wait();
+  griddep_launch();
   const int item = blockIdx.y, ty = 256 / tx;
   const T* src = (const T*)g.p + (long long)item * g.stride;
   const int units = g.rows / V, x0 = threadIdx.x % tx;  // V divides the rows
@@ -139,8 +141,8 @@ __device__ __forceinline__ void store_half(__half* at, long long plane, float v)
 template <typename T, int V, int PLANES>
 __global__ void __launch_bounds__(256) ingest_kernel(Matrices g, const double* parts, int n_parts, __half* x, long long ld, long long plane, int tx,
                                                      const __grid_constant__ Plan plan, float2* factors) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  griddep_wait();
+  griddep_launch();
   const int item = blockIdx.y, ty = 256 / tx, batch = gridDim.y;
   double sum = 0;
   for (int i = threadIdx.x; i < n_parts; i += 256) sum += parts[(long long)item * kNormParts + i];
@@ -459,18 +461,11 @@ int run(const blb200_newton_schulz_desc* d, const Layout& l, char* ws, cudaStrea
   const int most = sms * 8 / batch + 1;  // eight blocks per SM fill it
   const int n_parts = std::min(std::min(rows_of_blocks, most), kNormParts);
   auto passes = [&](auto norm, auto ingest) {
-    norm<<<dim3(n_parts, batch), 256, 0, stream>>>(g, parts, tx);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(std::min(rows_of_blocks, most), batch);
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const int e = (int)cudaLaunchKernelEx(&cfg, ingest, g, (const double*)parts, n_parts, x.p, l.ld_x, l.plane_x, tx, plan, factors);
-    return e ? e : (int)cudaGetLastError();
+    const OverlappedLaunch first(dim3(n_parts, batch), 256, stream);
+    const int e = (int)cudaLaunchKernelEx(&first.cfg, norm, g, parts, tx);
+    if (e) return e;
+    const OverlappedLaunch launch(dim3(std::min(rows_of_blocks, most), batch), 256, stream);
+    return (int)cudaLaunchKernelEx(&launch.cfg, ingest, g, (const double*)parts, n_parts, x.p, l.ld_x, l.plane_x, tx, plan, factors);
   };
   int rc = wide ? passes(norm_parts_kernel<T, V>, ingest_kernel<T, V, PLANES>) : passes(norm_parts_kernel<T, 1>, ingest_kernel<T, 1, PLANES>);
   Maps maps;

@@ -98,6 +98,8 @@ __device__ __forceinline__ unsigned column_max(unsigned top, int tx) {
 // blockDim / tx columns.  Memory is all that it costs: 8192 x 8192 bfloat16 moves 201 MB.
 template <typename T, int V, int PER>
 __global__ void __launch_bounds__(1024) quantize_kernel(QuantizeParams p, int tx) {
+  griddep_wait();
+  griddep_launch();
   const long long total = (long long)p.cols * p.batch;
   const long long w = (long long)blockIdx.x * (blockDim.x / tx) + threadIdx.x / tx;
   const bool live = w < total;
@@ -123,6 +125,8 @@ __global__ void __launch_bounds__(1024) quantize_kernel(QuantizeParams p, int tx
 // Columns longer than a block's registers: read twice, the second time mostly from L2.
 template <typename T, int V>
 __global__ void __launch_bounds__(1024) quantize_long_kernel(QuantizeParams p) {
+  griddep_wait();
+  griddep_launch();
   const long long item = blockIdx.x / p.cols, col = blockIdx.x - item * p.cols;
   const T* x = (const T*)p.x + item * p.sx + col * p.ldx;
   int8_t* q = p.q + item * p.sq + col * p.ldq;
@@ -153,16 +157,16 @@ int launch_quantize(const QuantizeParams& p, cudaStream_t stream) {
   const long long threads = (units + per - 1) / per;
   if (threads > 1024) {
     if (total > 0x7fffffffll) return BLB200_E_TOO_LARGE;
-    quantize_long_kernel<T, V><<<(unsigned)total, 1024, 0, stream>>>(p);
-    return (int)cudaGetLastError();
+    const OverlappedLaunch launch((unsigned)total, 1024, stream);
+    return (int)cudaLaunchKernelEx(&launch.cfg, quantize_long_kernel<T, V>, p);
   }
   const int tx = threads <= 32 ? 32 : (int)((threads + 31) / 32 * 32);
   const int columns = tx >= 256 ? 1 : 256 / tx;
   const long long grid = (total + columns - 1) / columns;
   if (grid > 0x7fffffffll) return BLB200_E_TOO_LARGE;
   auto kern = per == 1 ? quantize_kernel<T, V, 1> : per == 4 ? quantize_kernel<T, V, 4> : quantize_kernel<T, V, (V == 1 ? 16 : 4)>;
-  kern<<<(unsigned)grid, columns * tx, 0, stream>>>(p, tx);
-  return (int)cudaGetLastError();
+  const OverlappedLaunch launch((unsigned)grid, columns * tx, stream);
+  return (int)cudaLaunchKernelEx(&launch.cfg, kern, p, tx);
 }
 
 int validate_quantize(const blb200_quantize_desc* d) {

@@ -45,7 +45,7 @@ def newton_schulz(X, Y=None, steps=5, coefficients=QUINTIC, eps=1e-7, *, workspa
     :func:`newton_schulz_workspace_bytes` bytes) is given.  Asynchronous."""
     if Y is None:
         Y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
-    _same_device("batchlas_b200.newton_schulz", X, Y)
+    _same_device("batchlas_b200.newton_schulz", X.get_device(), Y)
     d = _desc(X, Y, steps, coefficients, eps)
     with torch.cuda.device(Y.device):
         need = int(load().blb200_newton_schulz_workspace_bytes(d))

@@ -21,55 +21,64 @@ from .gemm import Transpose
 FTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _same_device(where, *ts):
-    """The device index that all tensors share.  These calls are short, so their host side is kept short too: no device
-    guard or stream object is made where the current ones are the right ones."""
-    index = ts[0].get_device()
-    for t in ts:
-        if t.get_device() != index:
-            index = -1 if t.get_device() < 0 or index < 0 else -2
-            break
-    if index == -1:
+# These calls are short, so their host side is kept short too: plain integers instead of views, no device guard or stream
+# object where the current ones are the right ones.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _same_device(where, index, *ts):
+    """Raises unless every tensor is on CUDA device `index`, the first operand's."""
+    if index < 0 or any(t.get_device() < 0 for t in ts):
         raise RuntimeError(f"{where} needs CUDA tensors; there is no CPU path")
-    if index == -2:
+    if any(t.get_device() != index for t in ts):
         raise RuntimeError(f"{where}: operands are on different devices")
-    return index
 
 
 def _launch(index, stream, fn, desc):
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return _launch(index, stream, fn, desc)
-    check(fn(desc, torch.cuda.current_stream(index).cuda_stream if stream is None else stream))
+    status = fn(desc, _raw_stream(index) if stream is None else stream)
+    if status:
+        check(status)
 
 
 def _matrix(t):
     """(batch, cols, rows, ld, stride) of a column-major tensor."""
-    shape, st = t.shape, t.stride()
-    if len(shape) == 2:
-        batch, (cols, rows), (ld, inner), stride = 1, shape, st, 0
-    elif len(shape) == 3:
-        (batch, cols, rows), (stride, ld, inner) = shape, st
+    st = t.stride()
+    if len(st) == 2:
+        cols, rows = t.shape
+        ld, inner = st
+        if inner == 1 and cols > 1:
+            return 1, cols, rows, ld, 0
+        batch, stride = 1, 0
+    elif len(st) == 3:
+        batch, cols, rows = t.shape
+        stride, ld, inner = st
         if batch <= 1:
             stride = 0
     else:
         raise ValueError("expected a (batch, cols, rows) or (cols, rows) tensor")
     if rows > 1 and inner != 1:
         raise ValueError("rows must be contiguous (column-major storage)")
-    if cols <= 1:
-        ld = max(rows, 1, ld)
-    return batch, cols, rows, ld, stride
+    return batch, cols, rows, ld if cols > 1 else max(rows, 1, ld), stride
 
 
 def _scales(where, s, batch, size, shared=True):
     """Batch stride of a float scale vector per item, or of one vector for the whole batch."""
-    if s.dtype != torch.float32:
+    if s.dtype is not torch.float32:
         raise TypeError(f"{where}: scales must be float32")
-    shape, st = s.shape, s.stride()
-    items = 1 if len(shape) == 1 else shape[0]
-    if len(shape) not in (1, 2) or shape[-1] != size or (items != batch and not (shared and items == 1)):
+    st = s.stride()
+    if len(st) == 1:
+        items, given, inner = 1, s.shape[0], st[0]
+    elif len(st) == 2:
+        items, given = s.shape
+        inner = st[1]
+    else:
+        given = -1
+    if given != size or (items != batch and not (shared and items == 1)):
         raise RuntimeError(f"{where}: incompatible scale dimensions")
-    if size > 1 and st[-1] != 1:
+    if inner != 1 and size > 1:
         raise ValueError(f"{where}: scales must be contiguous along the columns")
     return st[0] if items > 1 else 0
 
@@ -81,11 +90,13 @@ def quantize_i8(X, Q=None, scale=None, stream=None):
         Q = torch.empty(X.shape, dtype=torch.int8, device=X.device)
     if scale is None:
         scale = torch.empty(X.shape[:-1], dtype=torch.float32, device=X.device)
-    index = _same_device("batchlas_b200.quantize_i8", X, Q, scale)
+    index = X.get_device()
+    if index < 0 or Q.get_device() != index or scale.get_device() != index:
+        _same_device("batchlas_b200.quantize_i8", index, Q, scale)
     ftype = FTYPE_CODES.get(X.dtype)
     if ftype is None:
         raise TypeError("quantize_i8: X must be float32, float16 or bfloat16")
-    if Q.dtype != torch.int8:
+    if Q.dtype is not torch.int8:
         raise TypeError("quantize_i8: Q must be int8")
     batch, cols, k, ldx, stride_x = _matrix(X)
     q_batch, q_cols, q_k, ldq, stride_q = _matrix(Q)
@@ -104,8 +115,9 @@ def gemm_i8(A, B, C, scale_a=None, scale_b=None, alpha=1.0, beta=0.0, transA: Tr
     A (k x m) and B (k x n) are int8 with k fastest, so the op pair is always (Trans, NoTrans); C (m x n) is float32,
     float16 or bfloat16.  scale_a has one float per row of C (channel), scale_b one per column (token); one vector may
     serve the whole batch, None stands for ones.  A or B of batch 1 likewise serve every item of C."""
-    index = _same_device("batchlas_b200.gemm_i8", C, A, B, *(t for t in (scale_a, scale_b) if t is not None))
-    if A.dtype != torch.int8 or B.dtype != torch.int8:
+    index = C.get_device()
+    _same_device("batchlas_b200.gemm_i8", index, A, B, *(t for t in (scale_a, scale_b) if t is not None))
+    if A.dtype is not torch.int8 or B.dtype is not torch.int8:
         raise TypeError("gemm_i8: A and B must be int8")
     ftype = FTYPE_CODES.get(C.dtype)
     if ftype is None:

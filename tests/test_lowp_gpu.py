@@ -122,7 +122,7 @@ def bl_name():
 
 
 SHAPES = [(1, 1, 1, 1), (1, 1, 16, 3), (7, 5, 3, 2), (16, 1, 32, 1), (128, 1, 256, 1), (129, 17, 130, 2), (256, 16, 4096, 1),
-          (512, 33, 2048, 2), (300, 257, 1000, 1), (64, 500, 48, 2), (640, 384, 512, 1), (1000, 96, 128, 5), (40, 8, 8192, 1),
+          (512, 33, 2048, 2), (300, 257, 1000, 1), (64, 500, 48, 2), (640, 384, 512, 1), (1000, 96, 128, 5), (40, 8, 8192, 1), (200, 32, 1040, 2), (17, 24, 190, 3),
           (2048, 3, 400, 1), (257, 1024, 272, 1), (128, 128, 16, 2), (1, 700, 640, 1), (700, 1, 640, 1), (513, 130, 96, 3), (2305, 2300, 160, 1),
           (500, 300, 272, 20)]
 
