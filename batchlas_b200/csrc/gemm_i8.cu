@@ -1,10 +1,8 @@
 // 8-bit integer products with scales:  C <- alpha diag(sa) A^T B diag(sb) + beta C,  A (k x m) and B (k x n)
 // int8 with k fastest.  The sums are exact 32-bit integers, so every kernel here gives the same bits.
-//
-// Tile kernel for any alignment: 128 x 128 of C per CTA, eight warps of 32 x 64, mma.sync m16n8k32 on
-// 64-byte k chunks staged in shared memory (pitch 80 bytes: the eight rows of a fragment request fall
-// into different banks).  Rows that start off a 4-byte boundary are read as aligned words and shifted
-// together; a word is read whole only where all of it lies inside the operand.
+#include <math.h>
+
+#include <algorithm>
 #include <type_traits>
 
 #include "lowp.cuh"
@@ -32,32 +30,6 @@ __device__ __forceinline__ void store_c(T* c, int acc, float sa, float sb, float
   *c = from_f32<T>(v);
 }
 
-constexpr int kTile = 128, kChunk = 64, kPitch = 80;
-
-// 16 bytes at `src` (any alignment) of which the first `valid` exist, the rest zero.  [lo, hi) is the operand.
-__device__ __forceinline__ uint4 load16_any(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (valid >= 16) {
-    const int off = (int)(reinterpret_cast<uintptr_t>(src) & 3u);
-    const int8_t* base = src - off;
-    if (off == 0) {
-      const uint32_t* s = reinterpret_cast<const uint32_t*>(base);
-      return make_uint4(s[0], s[1], s[2], s[3]);
-    }
-    if (base >= lo && base + 20 <= hi) {
-      const uint32_t* s = reinterpret_cast<const uint32_t*>(base);
-      const uint32_t x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3], x4 = s[4];
-      const int sh = off * 8;
-      return make_uint4(__funnelshift_r(x0, x1, sh), __funnelshift_r(x1, x2, sh), __funnelshift_r(x2, x3, sh),
-                        __funnelshift_r(x3, x4, sh));
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (i < valid) w[i >> 2] |= (uint32_t)(uint8_t)src[i] << (8 * (i & 3));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 __device__ __forceinline__ void mma_i8(int (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -65,109 +37,8 @@ __device__ __forceinline__ void mma_i8(int (&d)[4], const uint32_t (&a)[4], cons
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_i8_any_kernel(GemmI8Params p, int tiles_m, long long tiles_per_item, long long tiles) {
-  __shared__ __align__(16) unsigned char tile_a[kTile * kPitch];
-  __shared__ __align__(16) unsigned char tile_b[kTile * kPitch];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int wm = (warp & 3) * 32, wn = (warp >> 2) * 64;
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const long long item = tile / tiles_per_item;
-    const int rem = (int)(tile - item * tiles_per_item);
-    const int m0 = rem % tiles_m * kTile, n0 = rem / tiles_m * kTile;
-    const int8_t* a = p.a + item * p.sa;
-    const int8_t* b = p.b + item * p.sb;
-    const int8_t* a_end = a + (long long)(p.m - 1) * p.lda + p.k;
-    const int8_t* b_end = b + (long long)(p.n - 1) * p.ldb + p.k;
-    int acc[2][8][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0;
-    uint4 next[4];
-    auto fetch = [&](int k0) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int c = tid + (u & 1) * 256, row = c >> 2, kk = k0 + (c & 3) * 16;
-        const bool is_a = u < 2;
-        const int r = (is_a ? m0 : n0) + row;
-        const int valid = r < (is_a ? p.m : p.n) ? p.k - kk : 0;
-        next[u] = valid > 0 ? load16_any((is_a ? a + (long long)r * p.lda : b + (long long)r * p.ldb) + kk, valid,
-                                         is_a ? a : b, is_a ? a_end : b_end)
-                            : make_uint4(0, 0, 0, 0);
-      }
-    };
-    fetch(0);
-    for (int k0 = 0; k0 < p.k; k0 += kChunk) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int c = tid + (u & 1) * 256;
-        *reinterpret_cast<uint4*>((u < 2 ? tile_a : tile_b) + (c >> 2) * kPitch + (c & 3) * 16) = next[u];
-      }
-      __syncthreads();
-      if (k0 + kChunk < p.k) fetch(k0 + kChunk);
-#pragma unroll
-      for (int ks = 0; ks < kChunk; ks += 32) {
-        uint32_t fa[2][4], fb[8][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const unsigned char* s = tile_a + (wm + i * 16 + g) * kPitch + ks + t * 4;
-          fa[i][0] = *reinterpret_cast<const uint32_t*>(s);
-          fa[i][1] = *reinterpret_cast<const uint32_t*>(s + 8 * kPitch);
-          fa[i][2] = *reinterpret_cast<const uint32_t*>(s + 16);
-          fa[i][3] = *reinterpret_cast<const uint32_t*>(s + 8 * kPitch + 16);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const unsigned char* s = tile_b + (wn + j * 8 + g) * kPitch + ks + t * 4;
-          fb[j][0] = *reinterpret_cast<const uint32_t*>(s);
-          fb[j][1] = *reinterpret_cast<const uint32_t*>(s + 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) mma_i8(acc[i][j], fa[i], fb[j]);
-      }
-      __syncthreads();
-    }
-    T* c = (T*)p.c + item * p.sc;
-    const float* sa = p.scale_a ? p.scale_a + item * p.ssa : nullptr;
-    const float* sb = p.scale_b ? p.scale_b + item * p.ssb : nullptr;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = m0 + wm + i * 16 + h * 8 + g;
-        if (row >= p.m) continue;
-        const float fsa = sa ? sa[row] : 1.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int col = n0 + wn + j * 8 + t * 2 + e;
-            if (col < p.n)
-              store_c(c + (long long)col * p.ldc + row, acc[i][j][h * 2 + e], fsa, sb ? sb[col] : 1.f, p.alpha, p.beta);
-          }
-      }
-  }
-}
-
-int launch_gemm_i8_any(const GemmI8Params& p, int ftype, cudaStream_t stream) {
-  const int tiles_m = (p.m + kTile - 1) / kTile;
-  const long long per_item = (long long)tiles_m * ((p.n + kTile - 1) / kTile), tiles = per_item * p.batch;
-  const long long cap = (long long)device_info().sm_count * 2;
-  return with_ftype(ftype, [&](auto t) {
-    gemm_i8_any_kernel<decltype(t)><<<(unsigned)(tiles < cap ? tiles : cap), 256, 0, stream>>>(p, tiles_m, per_item, tiles);
-    const int e = (int)cudaGetLastError();
-    if (e == 0) note_launch("gemm_i8_any");
-    return e;
-  });
-}
-
 // ---- few columns -----------------------------------------------------------------------------------
-// Up to 32 tokens: the weights are read once and that is the time.  A CTA owns MT tiles of 16 rows of C; its eight warps
+// Up to 16 tokens: the weights are read once and that is the time.  A CTA owns MT tiles of 16 rows of C; its eight warps
 // split k, and every lane holds its share of a 16 x 64 slab of weights by two 16-byte loads straight into mma.sync
 // fragments: the order of k inside a slab does not matter as long as both operands share it, so lane (g, t) takes bytes
 // 16 t .. 16 t + 15 of rows g and g + 8 (and of token g), words 0, 1 for one instruction and 2, 3 for the next.  The slabs of
@@ -175,13 +46,14 @@ int launch_gemm_i8_any(const GemmI8Params& p, int ftype, cudaStream_t stream) {
 // the tokens are read (from L2); the fewer, the more SMs take part.  Before it waits for the kernel that produced
 // its tokens, each lane asks for its first weights to be brought into L2, which has no effect but on time.  The warps' sums
 // meet in shared memory.
-constexpr int kFlight = 4;
+constexpr int kFlight = 4, kFewColumns = 16;
 
 template <bool WHOLE>
 __device__ __forceinline__ uint4 load16(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
   if (WHOLE && valid >= 16) return *reinterpret_cast<const uint4*>(src);
   if (valid <= 0) return make_uint4(0, 0, 0, 0);
-  return load16_any(src, valid, lo, hi);
+  const Words16 w = load16_words(src, valid, lo, hi);
+  return w.edge ? load16_bytes(src, valid) : w.v;
 }
 
 // WHOLE: both operands' columns start on 16-byte boundaries.
@@ -291,8 +163,7 @@ int launch_gemm_i8_few(const GemmI8Params& p, int ftype, cudaStream_t stream) {
                        : with_rows(nt, std::integral_constant<int, 1>{});
     };
     const cudaError_t e = p.n <= 8    ? with_columns(std::integral_constant<int, 1>{})
-                          : p.n <= 16 ? with_columns(std::integral_constant<int, 2>{})
-                                      : with_columns(std::integral_constant<int, 4>{});
+                                      : with_columns(std::integral_constant<int, 2>{});
     if (e == cudaSuccess) note_launch("gemm_i8_few");
     return (int)e;
   });
@@ -304,36 +175,78 @@ int launch_gemm_i8_few(const GemmI8Params& p, int ftype, cudaStream_t stream) {
 // column of C.
 enum { kUmmaI8Wait = 500 };
 
-template <typename T>
+struct I8Params {
+  GemmI8Params g;
+  int ftype;
+};
+
 struct I8Epilogue {
-  using Params = GemmI8Params;
-  T* c;
-  const float* sb;
-  const Params& p;
+  using Params = I8Params;
+  static constexpr bool kStaged = false;
+  template <int W>
+  struct Tile;
+};
+template <int W>
+struct I8Epilogue::Tile {
+  const I8Params& p;
+  long long item, m;
+  int n0;
   float sa;
   bool live;
-  __device__ I8Epilogue(const Params& p_, const UmmaShape&, const UmmaTile& tile, bool, int m) : p(p_), live(m < p_.m) {
-    c = (T*)p.c + (long long)tile.item * p.sc + m;
-    sa = p.scale_a && live ? p.scale_a[(long long)tile.item * p.ssa + m] : 1.f;
-    sb = p.scale_b ? p.scale_b + (long long)tile.item * p.ssb : nullptr;
+  __device__ Tile(const Params& p_, const UmmaShape&, const UmmaTile& tile, bool, int m_, int n, unsigned char*, int)
+      : p(p_), item(tile.item), m(m_), n0(n), live(m_ < p_.g.m) {
+    sa = p.g.scale_a && live ? p.g.scale_a[item * p.g.ssa + m] : 1.f;
   }
-  template <int N>
-  __device__ void store(const uint32_t (&v)[N], int n) {
-    if (!live) return;
-    T* at = c + (long long)n * p.ldc;
+  // Columns n0 + c ... n0 + c + W - 1 of the row.
+  __device__ __forceinline__ void group(const uint32_t (&v)[W], int c) {
+    const int n = n0 + c;
+    if (!live || n >= p.g.n) return;
+    if (p.ftype == BLB200_F32) store_as<float>(v, n);
+    else if (p.ftype == BLB200_F16) store_as<__half>(v, n);
+    else store_as<__nv_bfloat16>(v, n);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store_as(const uint32_t (&v)[W], int n) {
+    T* at = (T*)p.g.c + item * p.g.sc + m + (long long)n * p.g.ldc;
+    const float* sb = p.g.scale_b ? p.g.scale_b + item * p.g.ssb + n : nullptr;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (n + i < p.n) store_c(at + (long long)i * p.ldc, (int)v[i], sa, sb ? sb[n + i] : 1.f, p.alpha, p.beta);
+    for (int i = 0; i < W; ++i) {
+      if (n + i < p.g.n) store_c(at, (int)v[i], sa, sb ? sb[i] : 1.f, p.g.alpha, p.g.beta);
+      at += p.g.ldc;
+    }
   }
 };
 
-bool umma_i8_supported(const GemmI8Params& p) {
-  return p.k > 0 && columns_16(p.a, p.lda, p.sa, p.m, p.batch) && columns_16(p.b, p.ldb, p.sb, p.n, p.batch) && encode_tiled_fn() != nullptr;
+// Estimated time of one way to cut C into tiles, in SM cycles: rounds of tiles, each as long as the slower of its MMAs
+// (8192 products per cycle) and of its fetches (about 50 bytes per cycle and SM from L2), and about 2500 cycles for filling the ring
+// and the epilogue; splitting k costs an exchange of about 1500.
+struct TileChoice {
+  int group, bn, split;
+  double time;
+};
+double tile_time(const GemmI8Params& p, int group, int bn, int split) {
+  const long long sms = device_info().sm_count, bm = 128 * group;
+  const long long tiles = (p.m + bm - 1) / bm * ((p.n + bn - 1) / bn) * p.batch;
+  const double blocks = (double)((p.k + 127) / 128), per = std::max(2.0 * bn, (16384.0 + 128.0 * bn / group) / 50.0);
+  if (split > 1 && tiles * split > sms) return 1e300;
+  const double rounds = split > 1 ? 1.0 : (double)((tiles + sms / group - 1) / (sms / group));
+  return rounds * (ceil(blocks / split) * per + 2500.0) + (split > 1 ? 1500.0 : 0.0);
+}
+TileChoice choose_tiles(const GemmI8Params& p, bool aligned) {
+  TileChoice best{1, 128, 1, tile_time(p, 1, 128, 1)};
+  auto consider = [&](int group, int bn, int split) {
+    const double t = tile_time(p, group, bn, split);
+    if (t < best.time) best = TileChoice{group, bn, split, t};
+  };
+  for (int bn : {64, 128})
+    for (int split : {1, 2, 4, 8}) consider(1, bn, split);
+  if (aligned) consider(2, 256, 1);
+  return best;
 }
 
-template <int GROUP, int BN>
+template <int GROUP, int BN, int SPLIT, bool PLAIN>
 int launch_umma_i8(const GemmI8Params& p, int ftype, cudaStream_t stream) {
-  using C = UmmaConfig<true, false, false, GROUP, BN, 1>;
+  using C = UmmaConfig<true, false, false, GROUP, BN, 1, SPLIT, PLAIN>;
   UmmaShape s{};
   s.m = p.m;
   s.n = p.n;
@@ -341,24 +254,40 @@ int launch_umma_i8(const GemmI8Params& p, int ftype, cudaStream_t stream) {
   s.batch = p.batch;
   s.a_items = p.batch > 1 && p.sa == 0 ? 1 : p.batch;
   s.b_items = p.batch > 1 && p.sb == 0 ? 1 : p.batch;
-  // a single column's ld is not used for addressing, but the map wants a multiple of 16
-  auto ld_of = [](long long ld, int cols) { return cols == 1 ? (ld + 15) / 16 * 16 : ld; };
-  CUtensorMap map_a, map_b;
-  int rc = encode_operand(&map_a, p.a, true, p.k, p.m, s.a_items, ld_of(p.lda, p.m), p.sa, 128);
-  if (rc == BLB200_OK) rc = encode_operand(&map_b, p.b, true, p.k, p.n, s.b_items, ld_of(p.ldb, p.n), p.sb, C::kBRows);
-  if (rc != BLB200_OK) return rc;
-  return with_ftype(ftype, [&](auto t) {
-    const int e = launch_umma<C, I8Epilogue<decltype(t)>>(map_a, map_b, s, p, kUmmaI8Wait, stream);
-    if (e == 0) note_launch("gemm_i8_umma");
-    return e;
-  });
+  CUtensorMap map_a{}, map_b{};
+  if (!PLAIN) {
+    // a single column's ld is not used for addressing, but the map wants a multiple of 16
+    auto ld_of = [](long long ld, int cols) { return cols == 1 ? (ld + 15) / 16 * 16 : ld; };
+    int rc = encode_operand(&map_a, p.a, true, p.k, p.m, s.a_items, ld_of(p.lda, p.m), p.sa, 128);
+    if (rc == BLB200_OK) rc = encode_operand(&map_b, p.b, true, p.k, p.n, s.b_items, ld_of(p.ldb, p.n), p.sb, C::kBRows);
+    if (rc != BLB200_OK) return rc;
+  }
+  const PlainOperands po{p.a, p.b, p.lda, p.ldb, p.sa, p.sb};
+  const int e = launch_umma<C, I8Epilogue>(map_a, map_b, map_a, map_b, s, I8Params{p, ftype}, kUmmaI8Wait, stream, po);
+  if (e == 0) note_launch(PLAIN ? "gemm_i8_plain" : "gemm_i8_umma");
+  return e;
 }
 
-int launch_umma_i8_any(const GemmI8Params& p, int ftype, cudaStream_t stream) {
-  if (p.n <= 64) return launch_umma_i8<1, 64>(p, ftype, stream);
-  const long long pairs = (long long)((p.m + 255) / 256) * ((p.n + 255) / 256) * p.batch, units = device_info().sm_count / 2;
-  if (pairs >= units) return launch_umma_i8<2, 256>(p, ftype, stream);
-  return launch_umma_i8<1, 128>(p, ftype, stream);
+template <bool PLAIN>
+int launch_tiles_i8(const GemmI8Params& p, const TileChoice& c, int ftype, cudaStream_t stream) {
+  if constexpr (!PLAIN)
+    if (c.group == 2) return launch_umma_i8<2, 256, 1, false>(p, ftype, stream);
+#define BLB_TILE(BN_, SPLIT_) \
+  if (c.bn == BN_ && c.split == SPLIT_) return launch_umma_i8<1, BN_, SPLIT_, PLAIN>(p, ftype, stream);
+  BLB_TILE(64, 1) BLB_TILE(64, 2) BLB_TILE(64, 4) BLB_TILE(64, 8)
+  BLB_TILE(128, 1) BLB_TILE(128, 2) BLB_TILE(128, 4) BLB_TILE(128, 8)
+#undef BLB_TILE
+  return BLB200_E_INTERNAL;
+}
+
+int dispatch_gemm_i8(const GemmI8Params& p, int ftype, cudaStream_t stream) {
+  if (p.n <= kFewColumns && ((long long)(p.m + 15) / 16) * p.batch <= 0x7fffffffll) return launch_gemm_i8_few(p, ftype, stream);
+  const bool aligned = p.k > 0 && columns_16(p.a, p.lda, p.sa, p.m, p.batch) && columns_16(p.b, p.ldb, p.sb, p.n, p.batch);
+  if (aligned) {
+    const int rc = launch_tiles_i8<false>(p, choose_tiles(p, true), ftype, stream);
+    if (rc != BLB200_E_INTERNAL) return rc;  // a driver that refuses the tensor maps: plain loads take it
+  }
+  return launch_tiles_i8<true>(p, choose_tiles(p, false), ftype, stream);
 }
 
 constexpr int kMaxK = 131071;  // 128 * 128 * k stays below 2^31
@@ -389,11 +318,5 @@ extern "C" int blb200_gemm_i8(const blb200_gemm_i8_desc* d, void* cuda_stream) {
                  d->k,   d->batch, d->lda,    d->ldb,      d->ldc,      d->stride_a,    d->stride_b,
                  d->stride_c, d->stride_scale_a, d->stride_scale_b, (float)d->alpha, (float)d->beta};
   if (p.k == 0) p.scale_a = p.scale_b = nullptr;  // C <- beta * C, whatever the scales hold
-  if (p.n <= 32 && p.k > 0 && ((long long)(p.m + 15) / 16) * p.batch <= 0x7fffffffll)
-    return launch_gemm_i8_few(p, d->ftype_c, (cudaStream_t)cuda_stream);
-  if (umma_i8_supported(p)) {
-    const int e = launch_umma_i8_any(p, d->ftype_c, (cudaStream_t)cuda_stream);
-    if (e != BLB200_E_INTERNAL) return e;  // a driver that refuses the tensor map: the tile kernel takes it
-  }
-  return launch_gemm_i8_any(p, d->ftype_c, (cudaStream_t)cuda_stream);
+  return dispatch_gemm_i8(p, d->ftype_c, (cudaStream_t)cuda_stream);
 }

@@ -13,57 +13,18 @@
 // Layout: X keeps the caller's orientation (rows fastest), so nothing is transposed.  With rows <= cols the Gram product
 // contracts over the slow index (both operands MN-major) and the update over the fast one; with rows > cols the other
 // way round.  S and B are symmetric: tiles on and below the diagonal are computed and stored twice.
-#include <math.h>
-
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
-#include "lowp.cuh"
+#include "newton_schulz.cuh"
 #include "umma_gemm.cuh"
 
 namespace blb200 {
 namespace {
 
 enum { kUmmaNsWait = 600 };
-constexpr int kNormParts = 1024, kMaxSteps = 64;
-constexpr double kMaxSigma = 64.0, kMaxEntry = 16384.0;
-constexpr double kGrowth = 1.01;  // what the roundings of a step may add to the bound of X
-
-struct Matrices {
-  void* p;
-  int rows, cols, batch;
-  long long ld, stride;
-};
-
-// Largest |a s + b s^3 + c s^5| over 0 <= s <= top.
-__host__ __device__ inline double polynomial_bound(const double* q, double top) {
-  auto value = [&](double s) { return fabs(s * (q[0] + s * s * (q[1] + s * s * q[2]))); };
-  double best = value(top);
-  // critical points: a + 3 b t + 5 c t^2 = 0 with t = s^2
-  const double A = 5 * q[2], B = 3 * q[1], C = q[0], disc = B * B - 4 * A * C;
-  if (A == 0) {
-    if (B != 0 && -C / B > 0 && -C / B < top * top) best = fmax(best, value(sqrt(-C / B)));
-  } else if (disc >= 0) {
-    const double r = sqrt(disc);
-    for (int i = 0; i < 2; ++i) {
-      const double t = (-B + (i ? -r : r)) / (2 * A);
-      if (t > 0 && t < top * top) best = fmax(best, value(sqrt(t)));
-    }
-  }
-  return best;
-}
-
-__device__ __forceinline__ double block_sum(double v) {
-  __shared__ double part[8];
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0;
-  for (int i = 0; i < 8; ++i) v += part[i];
-  __syncthreads();
-  return v;
-}
-
+constexpr int kNormParts = 1024;
 // The passes over G: 256 threads as (256 / tx) columns of tx threads, each thread walking down its column in units of V
 // elements (16 bytes where the layout allows it, else single elements).
 template <typename T, int V>
@@ -101,34 +62,6 @@ __global__ void __launch_bounds__(256) norm_parts_kernel(Matrices g, double* par
   if (threadIdx.x == 0) parts[(long long)item * kNormParts + blockIdx.x] = sum;
 }
 
-// Power of two that takes a value of at most `top` below 2^15.
-__host__ __device__ inline double half_scale(double top) {
-  if (!(top > 0) || isinf(top)) return 1.0;
-  const int e = 14 - ilogb(top);
-  return scalbn(1.0, e > 400 ? 400 : e);
-}
-
-// The powers of two that S, B and the next X are stored with at one step, from the bound of X before it.
-struct StepScales {
-  double s, b, next;
-};
-__host__ __device__ inline StepScales step_scales(const double* q, double& sigma, bool last) {
-  const double s2 = sigma * sigma;
-  StepScales r;
-  r.s = half_scale(s2);
-  r.b = half_scale(fabs(q[1]) * s2 + fabs(q[2]) * s2 * s2);
-  sigma = polynomial_bound(q, sigma) * kGrowth;
-  r.next = last ? 1.0 : half_scale(sigma);
-  return r;
-}
-
-struct Plan {
-  double q[3 * kMaxSteps];        // coefficients, by step
-  StepScales scales[kMaxSteps];   // for a matrix that starts with |X| <= 1
-  double eps;
-  int steps;
-};
-
 template <int PLANES>
 __device__ __forceinline__ void store_half(__half* at, long long plane, float v) {
   const __half hi = __float2half_rn(v);
@@ -147,35 +80,12 @@ __global__ void __launch_bounds__(256) ingest_kernel(Matrices g, const double* p
   double sum = 0;
   for (int i = threadIdx.x; i < n_parts; i += 256) sum += parts[(long long)item * kNormParts + i];
   sum = block_sum(sum);
-  const double norm = sqrt(sum), f = norm + plan.eps;
-  const bool usable = isfinite(sum) && f > 0;
-  const int e = sum > 0 && usable ? 14 - ilogb(norm) : 0;
-  const float t1 = usable ? scalbnf(1.f, e / 2) : __int_as_float(0x7fffffff), t2 = scalbnf(1.f, e - e / 2);
+  const ItemScale scale(sum, plan.eps);
+  const float t1 = scale.t1, t2 = scale.t2;
 
   if (blockIdx.x == 0) {
     __shared__ StepScales own[kMaxSteps];
-    // X = stored / (t f).  The bounds for |X| <= 1 hold for every item; one that eps makes much smaller gets its own, so
-    // that its matrices do not sink towards half's smallest numbers.
-    const bool small = norm < 0.125 * f;
-    if (small) {
-      if (threadIdx.x == 0) {
-        double sigma = norm / f;
-        for (int i = 0; i < plan.steps; ++i) own[i] = step_scales(plan.q + 3 * i, sigma, i + 1 == plan.steps);
-      }
-      __syncthreads();
-    }
-    const int i = threadIdx.x;
-    if (i < plan.steps) {
-      const StepScales* sc = small ? own : plan.scales;
-      const double ss = sc[i].s, sb = sc[i].b, sn = sc[i].next;
-      // a zero item stays zero under any finite factors
-      const double sx = i > 0 ? sc[i - 1].next : (norm > 0 ? scalbn(1.0, e) * f : 1.0);
-      const double* q = plan.q + 3 * i;
-      float2* out = factors + (long long)i * 3 * batch + item;
-      out[0] = make_float2((float)(ss / sx / sx), 0.f);
-      out[batch] = make_float2((float)(q[2] * (sb / ss / ss)), (float)(q[1] * (sb / ss)));
-      out[2 * batch] = make_float2((float)(sn / sb / sx), (float)(q[0] * (sn / sx)));
-    }
+    write_factors(plan, scale.norm, scale.f, scale.e, own, factors + item, batch);
   }
 
   const T* src = (const T*)g.p + (long long)item * g.stride;
@@ -206,115 +116,96 @@ __global__ void __launch_bounds__(256) ingest_kernel(Matrices g, const double* p
   }
 }
 
-__device__ __forceinline__ uint32_t pack_halves(__half a, __half b) {
-  return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(b) << 16;
-}
-__device__ __forceinline__ __half half_of(uint32_t pair, int which) { return __ushort_as_half((unsigned short)(pair >> (16 * which))); }
-
-// out = alpha * product + beta * old, written as half planes (mirrored across the diagonal when the result is
-// symmetric) or, by the last step, in the caller's type and layout.
+// out = alpha * product + beta * old, left as half planes in the staging buffer (and stored across the diagonal as well when
+// the result is symmetric) or, by the last step, written in the caller's type and layout.
 template <typename T, int PLANES, bool LAST>
 struct NsEpilogue {
   struct Params {
     const float2* factors;
-    const __half* old;  // null: beta is not used
+    int has_old;  // 0: beta is not used
     void* out;
-    long long old_ld, old_plane, out_ld, out_plane, out_item;
+    long long out_ld, out_plane, out_item;
   };
-  const Params& p;
-  const UmmaShape& s;
-  const __half* old;
-  T* out;
-  T* mirror;
-  float alpha, beta;
-  bool live;
-  __device__ NsEpilogue(const Params& p_, const UmmaShape& s_, const UmmaTile& tile, bool twice, int m) : p(p_), s(s_), live(m < s_.m) {
-    const float2 f = p.factors[tile.item];
-    alpha = f.x;
-    beta = f.y;
-    old = p.old ? p.old + (long long)tile.item * PLANES * p.old_plane + m : nullptr;
-    T* base = (T*)p.out + (long long)tile.item * p.out_item;
-    out = base + m;
-    mirror = twice ? base + (long long)m * p.out_ld : nullptr;
-  }
-  // kGroup columns at a time: their old values are requested together (for pairs eight, or the sums spill).
-  static constexpr int kGroup = PLANES == 2 ? 8 : 16;
-  template <int N>
-  __device__ void store(const uint32_t (&v)[N], int n) {
-    if (!live) return;
-#pragma unroll
-    for (int g = 0; g < N; g += kGroup) {
-      if (n + g + kGroup <= s.n) store_group<N, true>(v, g, n + g);
-      else if (n + g < s.n) store_group<N, false>(v, g, n + g);
+  static constexpr bool kStaged = true, kStagedOut = !LAST;
+  // One thread's row of a tile, from column n0 on; `staged` is its element of column n0 in the staging buffer.
+  template <int W>
+  struct Tile {
+    const Params& p;
+    const UmmaShape& s;
+    T* out;
+    T* mirror;
+    __half* staged;
+    int plane;
+    float alpha, beta;
+    int n0;
+    bool live;
+    __device__ __forceinline__ Tile(const Params& p_, const UmmaShape& s_, const UmmaTile& tile, bool twice, int m, int n, unsigned char* staged_,
+                                    int plane_bytes)
+        : p(p_), s(s_), staged(reinterpret_cast<__half*>(staged_)), plane(plane_bytes / 2), n0(n), live(m < s_.m) {
+      const float2 f = p.factors[tile.item];
+      alpha = f.x;
+      beta = p.has_old ? f.y : 0.f;
+      T* base = (T*)p.out + (long long)tile.item * p.out_item;
+      out = base + m;
+      mirror = twice && live ? base + (long long)m * p.out_ld : nullptr;
     }
-  }
-  template <int N, bool FULL>
-  __device__ __forceinline__ void store_group(const uint32_t (&v)[N], int g, int n) {
-    float r[kGroup];
-    if (old) {
-      const __half* at = old + (long long)n * p.old_ld;
-      __half hi[kGroup], lo[kGroup];
+    // Columns n0 + c ... n0 + c + W - 1.
+    __device__ __forceinline__ void group(const uint32_t (&v)[W], int c) {
+      const int n = n0 + c;
+      __half* at = staged + c * 128;
+      float r[W];
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        if (FULL || n + i < s.n) {
-          hi[i] = at[0];
-          if constexpr (PLANES == 2) lo[i] = at[p.old_plane];
+      for (int i = 0; i < W; ++i) {
+        r[i] = alpha * __uint_as_float(v[i]);
+        if (p.has_old) {
+          float was = __half2float(at[i * 128]);
+          if constexpr (PLANES == 2) was += __half2float(at[plane + i * 128]);
+          r[i] = fmaf(beta, was, r[i]);
         }
-        at += p.old_ld;
       }
+      if constexpr (LAST) {
+        if (!live) return;
+        T* to = out + (long long)n * p.out_ld;
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        float was = __half2float(hi[i]);
-        if constexpr (PLANES == 2) was += __half2float(lo[i]);
-        r[i] = fmaf(beta, was, alpha * __uint_as_float(v[g + i]));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) r[i] = alpha * __uint_as_float(v[g + i]);
-    }
-    T* at = out + (long long)n * p.out_ld;
-    if constexpr (LAST) {
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        if (FULL || n + i < s.n) *at = from_f32<T>(r[i]);
-        at += p.out_ld;
-      }
-    } else {
-      uint32_t hi[kGroup / 2], lo[kGroup / 2];  // pairs of halves
-#pragma unroll
-      for (int i = 0; i < kGroup / 2; ++i) {
-        const __half h0 = __float2half_rn(r[2 * i]), h1 = __float2half_rn(r[2 * i + 1]);
-        hi[i] = pack_halves(h0, h1);
-        if constexpr (PLANES == 2)
-          lo[i] = pack_halves(__float2half_rn(r[2 * i] - __half2float(h0)), __float2half_rn(r[2 * i + 1] - __half2float(h1)));
-      }
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        if (FULL || n + i < s.n) {
-          at[0] = half_of(hi[i / 2], i & 1);
-          if constexpr (PLANES == 2) at[p.out_plane] = half_of(lo[i / 2], i & 1);
+        for (int i = 0; i < W; ++i) {
+          if (n + i < s.n) *to = from_f32<T>(r[i]);
+          to += p.out_ld;
         }
-        at += p.out_ld;
-      }
-      if (mirror) {
-        if (FULL) {
+      } else {
+        uint32_t hi[W / 2], lo[W / 2];  // pairs of halves
 #pragma unroll
-          for (int h = 0; h < kGroup / 2; h += 4) {
-            *reinterpret_cast<uint4*>(mirror + n + 2 * h) = make_uint4(hi[h], hi[h + 1], hi[h + 2], hi[h + 3]);
-            if constexpr (PLANES == 2)
-              *reinterpret_cast<uint4*>(mirror + p.out_plane + n + 2 * h) = make_uint4(lo[h], lo[h + 1], lo[h + 2], lo[h + 3]);
+        for (int i = 0; i < W; i += 2) {
+          const __half h0 = __float2half_rn(r[i]), h1 = __float2half_rn(r[i + 1]);
+          at[i * 128] = h0;
+          at[(i + 1) * 128] = h1;
+          hi[i / 2] = pack_halves(h0, h1);
+          if constexpr (PLANES == 2) {
+            const __half l0 = __float2half_rn(r[i] - __half2float(h0)), l1 = __float2half_rn(r[i + 1] - __half2float(h1));
+            at[plane + i * 128] = l0;
+            at[plane + (i + 1) * 128] = l1;
+            lo[i / 2] = pack_halves(l0, l1);
           }
-        } else {
+        }
+        if (mirror) {
 #pragma unroll
-          for (int i = 0; i < kGroup; ++i)
-            if (n + i < s.n) {
-              mirror[n + i] = half_of(hi[i / 2], i & 1);
-              if constexpr (PLANES == 2) mirror[p.out_plane + n + i] = half_of(lo[i / 2], i & 1);
+          for (int h = 0; h < W / 2; h += 4) {
+            if (n + 2 * h + 8 <= s.n) {
+              *reinterpret_cast<uint4*>(mirror + n + 2 * h) = make_uint4(hi[h], hi[h + 1], hi[h + 2], hi[h + 3]);
+              if constexpr (PLANES == 2)
+                *reinterpret_cast<uint4*>(mirror + p.out_plane + n + 2 * h) = make_uint4(lo[h], lo[h + 1], lo[h + 2], lo[h + 3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (n + 2 * h + i < s.n) {
+                  mirror[n + 2 * h + i] = half_of(hi[h + i / 2], i & 1);
+                  if constexpr (PLANES == 2) mirror[p.out_plane + n + 2 * h + i] = half_of(lo[h + i / 2], i & 1);
+                }
             }
+          }
         }
       }
     }
-  }
+  };
 };
 
 struct HalfMatrix {  // [item][plane][outer][ld], inner fastest
@@ -327,61 +218,77 @@ struct HalfMatrix {  // [item][plane][outer][ld], inner fastest
 struct Maps {
   struct Entry {
     const void* p;
-    int box;
+    int box, staged;
     CUtensorMap map;
   };
   Entry e[16];
   int used = 0;
-  int get(const CUtensorMap** out, const HalfMatrix& a, int z, int box) {
+  int get(const CUtensorMap** out, const HalfMatrix& a, int z, int box, int staged = 0) {
     for (int i = 0; i < used; ++i)
-      if (e[i].p == a.p && e[i].box == box) {
+      if (e[i].p == a.p && e[i].box == box && e[i].staged == staged) {
         *out = &e[i].map;
         return BLB200_OK;
       }
-    if (used == 16) return BLB200_E_INTERNAL;  // four matrices in three boxes each at most
-    const int rc = encode_operand(&e[used].map, a.p, false, a.inner, a.outer, z, a.ld * 2, a.plane * 2, box);
+    if (used == 16) return BLB200_E_INTERNAL;  // four matrices in four boxes each at most
+    const int rc = encode_operand(&e[used].map, a.p, false, a.inner, a.outer, z, a.ld * 2, a.plane * 2, box, staged != 0);
     if (rc != BLB200_OK) return rc;
     e[used].p = a.p;
     e[used].box = box;
+    e[used].staged = staged;
     *out = &e[used++].map;
     return BLB200_OK;
   }
 };
 
-template <bool A_MN, bool B_MN, int GROUP, int BN, int PLANES, class Epilogue>
-int launch_product(Maps& maps, const HalfMatrix& a, const HalfMatrix& b, int m, int n, int k, int batch, bool symmetric,
-                   const typename Epilogue::Params& ep, cudaStream_t stream) {
-  using C = UmmaConfig<false, A_MN, B_MN, GROUP, BN, PLANES>;
+struct Operands {
+  HalfMatrix a, b, old, out;
+  int m, n, k, batch;
+  bool symmetric;
+};
+
+template <bool A_MN, bool B_MN, int GROUP, int BN, int PLANES, int SPLIT, class Epilogue>
+int launch_product(Maps& maps, const Operands& o, const typename Epilogue::Params& ep, cudaStream_t stream) {
+  using C = UmmaConfig<false, A_MN, B_MN, GROUP, BN, PLANES, SPLIT>;
   UmmaShape s{};
-  s.m = m;
-  s.n = n;
-  s.k = k;
-  s.batch = batch;
-  s.symmetric = symmetric;  // a_items, b_items stay 0: no operand is shared by the items
-  const CUtensorMap *map_a, *map_b;
-  int rc = maps.get(&map_a, a, batch * PLANES, A_MN ? 64 : 128);
-  if (rc == BLB200_OK) rc = maps.get(&map_b, b, batch * PLANES, B_MN ? 64 : C::kBRows);
-  if (rc == BLB200_OK) rc = launch_umma<C, Epilogue>(*map_a, *map_b, s, ep, kUmmaNsWait, stream);
+  s.m = o.m;
+  s.n = o.n;
+  s.k = o.k;
+  s.batch = o.batch;
+  s.symmetric = o.symmetric;  // a_items, b_items stay 0: no operand is shared by the items
+  const CUtensorMap *map_a, *map_b, *map_old, *map_out;
+  const int z = o.batch * PLANES;
+  int rc = maps.get(&map_a, o.a, z, A_MN ? 64 : 128);
+  if (rc == BLB200_OK) rc = maps.get(&map_b, o.b, z, B_MN ? 64 : C::kBRows);
+  map_old = map_out = map_a;
+  if (rc == BLB200_OK && ep.has_old) rc = maps.get(&map_old, o.old, z, kStagedColumns, 1);
+  if (rc == BLB200_OK && Epilogue::kStagedOut) rc = maps.get(&map_out, o.out, z, kStagedColumns, 1);
+  if (rc == BLB200_OK) rc = launch_umma<C, Epilogue>(*map_a, *map_b, *map_old, *map_out, s, ep, kUmmaNsWait, stream);
   if (rc == BLB200_OK) note_launch("newton_schulz");
   return rc;
 }
 
-// Tiles of 256 rows on CTA pairs (256 columns wide, for float 128) or of 128 x 128 on single CTAs: whichever needs less
-// time for the number of rounds its tiles come to.
+// Tiles of 256 rows on CTA pairs (256 columns wide, for pairs of halves 128), of 128 x 128 on single CTAs, or of 128 x 128
+// with k split over two or four CTAs: whichever should take the least time, in units of about 0.3 us: per 64 k a tile of 128 x
+// 128 takes one (pairs of halves: two and a half), a pair's takes 1.3 (2.5), a tile's start and end 12, an exchange 6.
 template <bool A_MN, bool B_MN, int PLANES, class Epilogue>
-int product(Maps& maps, const HalfMatrix& a, const HalfMatrix& b, int m, int n, int k, int batch, bool symmetric,
-            const typename Epilogue::Params& ep, cudaStream_t stream) {
+int product(Maps& maps, const Operands& o, const typename Epilogue::Params& ep, cudaStream_t stream) {
   constexpr int kPairN = PLANES == 2 ? 128 : 256;
   auto tiles = [&](int t_m, int t_n) {
-    const int tm = (m + t_m - 1) / t_m, tn = (n + t_n - 1) / t_n;
-    const long long each = !symmetric ? (long long)tm * tn : t_m == t_n ? symmetric_tiles<1>(tm, tn) : symmetric_tiles<2>(tm, tn);
-    return each * batch;
+    const int tm = (o.m + t_m - 1) / t_m, tn = (o.n + t_n - 1) / t_n;
+    const long long each = !o.symmetric ? (long long)tm * tn : t_m == t_n ? symmetric_tiles<1>(tm, tn) : symmetric_tiles<2>(tm, tn);
+    return each * o.batch;
   };
-  const long long sms = device_info().sm_count;
-  const double pair = kPairN / 128 * (double)((tiles(256, kPairN) + sms / 2 - 1) / (sms / 2));
-  const double single = 1.15 * (double)((tiles(128, 128) + sms - 1) / sms);
-  return pair <= single ? launch_product<A_MN, B_MN, 2, kPairN, PLANES, Epilogue>(maps, a, b, m, n, k, batch, symmetric, ep, stream)
-                        : launch_product<A_MN, B_MN, 1, 128, PLANES, Epilogue>(maps, a, b, m, n, k, batch, symmetric, ep, stream);
+  const long long sms = device_info().sm_count, blocks = (o.k + 63) / 64;
+  auto rounds = [](long long n, long long units) { return (double)((n + units - 1) / units); };
+  const double block = PLANES == 2 ? 2.5 : 1.0, pair_block = PLANES == 2 ? 2.5 : 1.3;
+  const double pair = rounds(tiles(256, kPairN), sms / 2) * (blocks * pair_block + 12);
+  const double single = rounds(tiles(128, 128), sms) * (blocks * block + 12);
+  auto split = [&](int s) { return tiles(128, 128) * s > sms ? 1e300 : (double)((blocks + s - 1) / s) * block + 18; };
+  const double best = std::min(std::min(pair, single), std::min(split(2), split(4)));
+  if (best == pair) return launch_product<A_MN, B_MN, 2, kPairN, PLANES, 1, Epilogue>(maps, o, ep, stream);
+  if (best == single) return launch_product<A_MN, B_MN, 1, 128, PLANES, 1, Epilogue>(maps, o, ep, stream);
+  if (best == split(2)) return launch_product<A_MN, B_MN, 1, 128, PLANES, 2, Epilogue>(maps, o, ep, stream);
+  return launch_product<A_MN, B_MN, 1, 128, PLANES, 4, Epilogue>(maps, o, ep, stream);
 }
 
 int validate_ns(const blb200_newton_schulz_desc* d) {
@@ -437,14 +344,12 @@ Layout layout_of(const blb200_newton_schulz_desc* d) {
   return l;
 }
 
-template <typename T, int PLANES>
-int run(const blb200_newton_schulz_desc* d, const Layout& l, char* ws, cudaStream_t stream) {
-  const int r = d->rows, c = d->cols, p = l.p, batch = d->batch;
-  const Matrices g{const_cast<void*>(d->x), r, c, batch, d->ldx, d->stride_x};
-  double* parts = (double*)(ws + l.parts);
-  float2* factors = (float2*)(ws + l.factors);
-  HalfMatrix x{(__half*)(ws + l.x), r, c, l.ld_x, l.plane_x}, x2{(__half*)(ws + l.x2), r, c, l.ld_x, l.plane_x};
-  const HalfMatrix s{(__half*)(ws + l.s), p, p, l.ld_s, l.plane_s}, b{(__half*)(ws + l.b), p, p, l.ld_s, l.plane_s};
+// Small matrices need none, but are given some like the others, so that a caller has one rule.
+size_t workspace_need(const blb200_newton_schulz_desc* d) {
+  return newton_schulz_small_supported(d->rows, d->cols) ? 256 : layout_of(d).total;
+}
+
+Plan plan_of(const blb200_newton_schulz_desc* d) {
   Plan plan;
   plan.eps = d->eps;
   plan.steps = d->steps;
@@ -453,6 +358,18 @@ int run(const blb200_newton_schulz_desc* d, const Layout& l, char* ws, cudaStrea
     for (int j = 0; j < 3; ++j) plan.q[3 * i + j] = d->coefficients[(d->coefficient_sets == 1 ? 0 : 3 * i) + j];
     plan.scales[i] = step_scales(plan.q + 3 * i, sigma, i + 1 == d->steps);
   }
+  return plan;
+}
+
+template <typename T, int PLANES>
+int run(const blb200_newton_schulz_desc* d, const Layout& l, char* ws, cudaStream_t stream) {
+  const Plan plan = plan_of(d);
+  const int r = d->rows, c = d->cols, p = l.p, batch = d->batch;
+  const Matrices g{const_cast<void*>(d->x), r, c, batch, d->ldx, d->stride_x};
+  double* parts = (double*)(ws + l.parts);
+  float2* factors = (float2*)(ws + l.factors);
+  HalfMatrix x{(__half*)(ws + l.x), r, c, l.ld_x, l.plane_x}, x2{(__half*)(ws + l.x2), r, c, l.ld_x, l.plane_x};
+  const HalfMatrix s{(__half*)(ws + l.s), p, p, l.ld_s, l.plane_s}, b{(__half*)(ws + l.b), p, p, l.ld_s, l.plane_s};
   constexpr int V = 16 / sizeof(T);
   const bool wide = r % V == 0 && reinterpret_cast<uintptr_t>(d->x) % 16 == 0 && d->ldx % V == 0 && (d->stride_x % V == 0 || batch == 1);
   int tx = 8;
@@ -473,24 +390,22 @@ int run(const blb200_newton_schulz_desc* d, const Layout& l, char* ws, cudaStrea
   using Last = NsEpilogue<T, PLANES, true>;
   for (int i = 0; i < d->steps && rc == BLB200_OK; ++i) {
     const float2* f = factors + (long long)i * 3 * batch;
-    const typename Inner::Params gram{f, nullptr, s.p, 0, 0, l.ld_s, l.plane_s, PLANES * l.plane_s};
-    rc = r <= c ? product<true, true, PLANES, Inner>(maps, x, x, p, p, c, batch, true, gram, stream)
-                : product<false, false, PLANES, Inner>(maps, x, x, p, p, r, batch, true, gram, stream);
+    const typename Inner::Params gram{f, 0, s.p, l.ld_s, l.plane_s, PLANES * l.plane_s};
+    const Operands gram_o{x, x, s, s, p, p, r <= c ? c : r, batch, true};
+    rc = r <= c ? product<true, true, PLANES, Inner>(maps, gram_o, gram, stream) : product<false, false, PLANES, Inner>(maps, gram_o, gram, stream);
     if (rc != BLB200_OK) break;
-    const typename Inner::Params square{f + batch, s.p, b.p, l.ld_s, l.plane_s, l.ld_s, l.plane_s, PLANES * l.plane_s};
-    rc = product<false, false, PLANES, Inner>(maps, s, s, p, p, p, batch, true, square, stream);
+    const typename Inner::Params square{f + batch, 1, b.p, l.ld_s, l.plane_s, PLANES * l.plane_s};
+    rc = product<false, false, PLANES, Inner>(maps, Operands{s, s, s, b, p, p, p, batch, true}, square, stream);
     if (rc != BLB200_OK) break;
+    const Operands update_o{r <= c ? b : x, r <= c ? x : b, x, x2, r, c, p, batch, false};
     if (i + 1 < d->steps) {
-      const typename Inner::Params update{f + 2 * batch, x.p, x2.p, l.ld_x, l.plane_x, l.ld_x, l.plane_x, PLANES * l.plane_x};
-      rc = r <= c ? product<false, false, PLANES, Inner>(maps, b, x, r, c, p, batch, false, update, stream)
-                  : product<true, false, PLANES, Inner>(maps, x, b, r, c, p, batch, false, update, stream);
-      const HalfMatrix swap = x;
-      x = x2;
-      x2 = swap;
+      const typename Inner::Params update{f + 2 * batch, 1, x2.p, l.ld_x, l.plane_x, PLANES * l.plane_x};
+      rc = r <= c ? product<false, false, PLANES, Inner>(maps, update_o, update, stream)
+                  : product<true, false, PLANES, Inner>(maps, update_o, update, stream);
+      std::swap(x, x2);
     } else {
-      const typename Last::Params last{f + 2 * batch, x.p, d->y, l.ld_x, l.plane_x, d->ldy, 0, d->stride_y};
-      rc = r <= c ? product<false, false, PLANES, Last>(maps, b, x, r, c, p, batch, false, last, stream)
-                  : product<true, false, PLANES, Last>(maps, x, b, r, c, p, batch, false, last, stream);
+      const typename Last::Params last{f + 2 * batch, 1, d->y, d->ldy, 0, d->stride_y};
+      rc = r <= c ? product<false, false, PLANES, Last>(maps, update_o, last, stream) : product<true, false, PLANES, Last>(maps, update_o, last, stream);
     }
   }
   return rc;
@@ -503,7 +418,7 @@ int newton_schulz_device_status_clear() { return clear_device_status_word(); }
 
 extern "C" size_t blb200_newton_schulz_workspace_bytes(const blb200_newton_schulz_desc* d) {
   if (!d || d->rows <= 0 || d->cols <= 0 || d->batch <= 0) return 0;
-  return blb200::layout_of(d).total;
+  return blb200::workspace_need(d);
 }
 
 extern "C" int blb200_newton_schulz(const blb200_newton_schulz_desc* d, void* workspace, size_t workspace_bytes, void* cuda_stream) {
@@ -511,10 +426,14 @@ extern "C" int blb200_newton_schulz(const blb200_newton_schulz_desc* d, void* wo
   const int rc = validate_ns(d);
   if (rc != BLB200_OK) return rc;
   if (d->rows == 0 || d->cols == 0 || d->batch == 0) return BLB200_OK;
-  const Layout l = layout_of(d);
   if (!workspace) return BLB200_E_NULL;
-  if (workspace_bytes < l.total || reinterpret_cast<uintptr_t>(workspace) % 256) return BLB200_E_SHAPE;
+  if (workspace_bytes < workspace_need(d) || reinterpret_cast<uintptr_t>(workspace) % 256) return BLB200_E_SHAPE;
   cudaStream_t stream = (cudaStream_t)cuda_stream;
+  if (newton_schulz_small_supported(d->rows, d->cols)) {
+    const Matrices g{const_cast<void*>(d->x), d->rows, d->cols, d->batch, d->ldx, d->stride_x};
+    return launch_newton_schulz_small(g, Matrices{d->y, d->rows, d->cols, d->batch, d->ldy, d->stride_y}, d->ftype, plan_of(d), stream);
+  }
+  const Layout l = layout_of(d);
   if (d->ftype == BLB200_F32) return run<float, 2>(d, l, (char*)workspace, stream);
   if (d->ftype == BLB200_F16) return run<__half, 2>(d, l, (char*)workspace, stream);
   return run<__nv_bfloat16, 1>(d, l, (char*)workspace, stream);

@@ -15,6 +15,8 @@ int gemm_i8_device_status(int* out);
 int gemm_i8_device_status_clear();
 int newton_schulz_device_status(int* out);
 int newton_schulz_device_status_clear();
+int newton_schulz_small_device_status(int* out);
+int newton_schulz_small_device_status_clear();
 int small_device_status_clear();
 int gemv_ring_device_status_clear();
 int small_ring_device_status_clear();
@@ -70,6 +72,10 @@ extern "C" int blb200_device_status(int* out) {
   }
   if (word == 0) {
     rc = blb200::newton_schulz_device_status(&word);
+    if (rc != 0) return rc;
+  }
+  if (word == 0) {
+    rc = blb200::newton_schulz_small_device_status(&word);
     if (rc != 0) return rc;
   }
   if (word == 0) {

@@ -16,6 +16,17 @@
 // three products: 9.5e-6 of the iteration's result against 3e-6 for plain float sums); so for pairs only two k blocks (24
 // additions) are summed there, and the partial sums are added up in registers, rounded to nearest.
 //
+// SPLIT > 1: a cluster of SPLIT CTAs shares one output tile, each taking a range of k; their sums are exchanged through
+// distributed shared memory (the idle stages), each CTA adding up, in rank order, the columns that it stores.  For calls whose
+// tiles would leave most SMs without work.
+// PLAIN: the operands are not on 16-byte boundaries, so the eight epilogue warps fetch the stages themselves, as aligned words
+// shifted together and written where the swizzle puts them.
+//
+// Epilogue: a thread owns one row of the tile (32 consecutive rows per warp) and takes its columns in groups of sixteen, in a
+// rolled loop: unrolled over the tile the code is 10 KB and more, which a kernel of a few microseconds spends its time
+// fetching (128 x 128 tiles: 2.3 us of 5.6).  A staged epilogue reads the old values of the result's tile from, and leaves the new
+// ones in, a buffer of half columns (128 rows each) that tensor-map copies fill while the products run and write out.
+//
 // A wait that runs out records its code, and the role leaves its loop; the other roles' waits then run out as well, the
 // copies still in flight are waited for, tensor memory is freed and the kernel returns.
 #pragma once
@@ -28,15 +39,18 @@ namespace blb200 {
 struct UmmaShape {
   int m, n, k, batch;
   int tiles_m, tiles_n;
-  long long tiles;       // all tiles of the launch
+  int tiles;             // all tiles of the launch
   long long a_items, b_items;  // 1 when the operand is shared by the batch
   int symmetric;         // D is symmetric (m == n): tiles below the diagonal only
 };
 
-enum UmmaWait { kUmmaWaitEmpty = 1, kUmmaWaitFull = 2, kUmmaWaitAccFree = 3, kUmmaWaitAcc = 4, kUmmaWaitDrain = 5 };
+enum UmmaWait { kUmmaWaitEmpty = 1, kUmmaWaitFull = 2, kUmmaWaitAccFree = 3, kUmmaWaitAcc = 4, kUmmaWaitDrain = 5, kUmmaWaitStaging = 6, kUmmaWaitOld = 7 };
+constexpr int kStagedColumns = 32;  // columns per box of the staging buffer
 
-template <bool I8_, bool A_MN_, bool B_MN_, int GROUP_, int BN_, int PLANES_>
+template <bool I8_, bool A_MN_, bool B_MN_, int GROUP_, int BN_, int PLANES_, int SPLIT_ = 1, bool PLAIN_ = false>
 struct UmmaConfig {
+  static constexpr int SPLIT = SPLIT_;
+  static constexpr bool PLAIN = PLAIN_;
   static constexpr bool I8 = I8_, A_MN = A_MN_, B_MN = B_MN_;
   static constexpr int GROUP = GROUP_, BN = BN_, PLANES = PLANES_;
   static constexpr int kBM = 128 * GROUP;              // rows of a tile
@@ -45,14 +59,25 @@ struct UmmaConfig {
   static constexpr int kKStage = I8 ? 128 : 64;        // k per stage: 128 bytes
   static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;
   static constexpr int kStageBytes = PLANES * (kABytes + kBBytes);
-  static constexpr int kStages = (200 * 1024) / kStageBytes < 8 ? (200 * 1024) / kStageBytes : 8;
   static constexpr int kTmemColumns = 2 * BN < 32 ? 32 : 2 * BN;
   static constexpr int kThreads = 320;
   static constexpr int kChunk = PLANES == 2 ? 2 : 0;   // k blocks summed in tensor memory, 0 = all
   static constexpr int kRatio = kBM / BN;              // tile columns per tile row
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + 256;
+  static_assert(SPLIT == 1 || (GROUP == 1 && BN % (2 * SPLIT) == 0 && BN >= 32), "");
+  static_assert(!PLAIN || (I8 && GROUP == 1 && BN <= 128), "");
   static_assert(!I8 || (!A_MN && !B_MN && PLANES == 1), "8-bit operands are K-major");
-  static_assert(kStages >= 2 && kTmemColumns <= 512 && (kTmemColumns & (kTmemColumns - 1)) == 0, "");
+  static_assert(kTmemColumns <= 512 && (kTmemColumns & (kTmemColumns - 1)) == 0, "");
+};
+
+// Shared memory of one kernel: the ring, the exchange area of the epilogue, the barriers.
+template <class C, class Epilogue>
+struct UmmaMemory {
+  static constexpr int kStaging = Epilogue::kStaged ? C::PLANES * C::BN * 256 : 0;
+  static constexpr int kFit = (224 * 1024 - kStaging) / C::kStageBytes;
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr size_t kBytes = 1024 + kStaging + (size_t)kStages * C::kStageBytes + 256;
+  static_assert(kStages >= 2 && kBytes <= 227 * 1024, "");
+  static_assert(C::SPLIT == 1 || C::BN * 512 <= kStages * C::kStageBytes, "the exchanged sums have to fit in the stages");
 };
 
 struct UmmaTile {
@@ -62,27 +87,27 @@ struct UmmaTile {
 // rows, walked column by column; for a symmetric D the tiles that reach the diagonal or lie below it, row by row
 // (tile row i has R (i + 1) of them, R columns of tiles being as wide as one row of tiles is high).
 template <int R>
-__host__ __device__ inline long long symmetric_tiles(int tiles_m, int tiles_n) {
-  const long long full_rows = (long long)R * tiles_m * (tiles_m - 1) / 2, last = (long long)R * tiles_m;
-  return full_rows + (last < tiles_n ? last : tiles_n);
+__host__ __device__ inline int symmetric_tiles(int tiles_m, int tiles_n) {
+  const int last = R * tiles_m;
+  return R * tiles_m * (tiles_m - 1) / 2 + (last < tiles_n ? last : tiles_n);
 }
 template <int R>
-__device__ __forceinline__ UmmaTile umma_tile(const UmmaShape& s, long long t) {
+__device__ __forceinline__ UmmaTile umma_tile(const UmmaShape& s, int t) {
   UmmaTile r;
   if (s.symmetric) {
-    const long long per = symmetric_tiles<R>(s.tiles_m, s.tiles_n);
-    r.item = (int)(t / per);
-    const int f = (int)(t - (long long)r.item * per);
+    const int per = symmetric_tiles<R>(s.tiles_m, s.tiles_n);
+    r.item = t / per;
+    const int f = t - r.item * per;
     int i = (int)((sqrtf((8.f / R) * (float)f + 1.f) - 1.f) * 0.5f);
-    while ((long long)R * (i + 1) * (i + 2) / 2 <= f) ++i;
-    while ((long long)R * i * (i + 1) / 2 > f) --i;
+    while (R * (i + 1) * (i + 2) / 2 <= f) ++i;
+    while (R * i * (i + 1) / 2 > f) --i;
     r.tm = i;
-    r.tn = f - (int)((long long)R * i * (i + 1) / 2);
+    r.tn = f - R * i * (i + 1) / 2;
     return r;
   }
-  const long long per = (long long)s.tiles_m * s.tiles_n;
-  r.item = (int)(t / per);
-  const int f = (int)(t - (long long)r.item * per);
+  const int per = s.tiles_m * s.tiles_n;
+  r.item = t / per;
+  const int f = t - r.item * per;
   constexpr int kBand = 8;
   const int band = f / (kBand * s.tiles_n), first = band * kBand;
   const int height = min(kBand, s.tiles_m - first);
@@ -92,33 +117,95 @@ __device__ __forceinline__ UmmaTile umma_tile(const UmmaShape& s, long long t) {
   return r;
 }
 
+// Operands that are fetched with plain loads (8-bit, K-major).
+struct PlainOperands {
+  const int8_t* a;
+  const int8_t* b;
+  long long lda, ldb, sa, sb;
+};
+
+// 16 bytes at `src` (any alignment) of which the first `valid` (at least 1) exist, the rest zero.  [lo, hi) is the operand: aligned
+// words that lie inside it are read whole and shifted together, without branches, so that many such loads can be in flight;
+// `edge` says that a word reaches over one of its ends, and load16_bytes has to do it.
+struct Words16 {
+  uint4 v;
+  bool edge;
+};
+__device__ __forceinline__ Words16 load16_words(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
+  const int off = (int)(reinterpret_cast<uintptr_t>(src) & 3u);
+  const int8_t* base = src - off;
+  uint32_t x[5];
+  bool edge = false;
+#pragma unroll
+  for (int j = 0; j < 5; ++j) {
+    const bool needed = 4 * j - off < min(valid, 16), inside = base + 4 * j >= lo && base + 4 * j + 4 <= hi;
+    x[j] = 0;
+    if (needed && inside) x[j] = *reinterpret_cast<const uint32_t*>(base + 4 * j);
+    edge |= needed && !inside;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    w[j] = __funnelshift_r(x[j], x[j + 1], off * 8);
+    const int left = valid - 4 * j;
+    if (left < 4) w[j] &= left > 0 ? 0xffffffffu >> (8 * (4 - left)) : 0u;
+  }
+  return Words16{make_uint4(w[0], w[1], w[2], w[3]), edge};
+}
+static __device__ __noinline__ uint4 load16_bytes(const int8_t* src, int valid) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int i = 0; i < 16 && i < valid; ++i) {
+    const uint32_t byte = (uint32_t)(uint8_t)src[i] << (8 * (i & 3));
+    if (i < 4) w[0] |= byte;
+    else if (i < 8) w[1] |= byte;
+    else if (i < 12) w[2] |= byte;
+    else w[3] |= byte;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <class C, class Epilogue>
 __global__ void __launch_bounds__(C::kThreads, 1)
-    umma_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const UmmaShape s,
-                     const typename Epilogue::Params ep, int wait_code) {
-  constexpr int S = C::kStages, G = C::GROUP;
+    umma_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                     const __grid_constant__ CUtensorMap map_old, const __grid_constant__ CUtensorMap map_out, const UmmaShape s,
+                     const typename Epilogue::Params ep, const PlainOperands po, int wait_code) {
+  using M = UmmaMemory<C, Epilogue>;
+  constexpr int S = M::kStages, G = C::GROUP;
+  constexpr int kCluster = G * C::SPLIT;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * C::kStageBytes);
+  unsigned char* staging = smem + (size_t)S * C::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + M::kStaging);
   uint64_t* empty = full + S;
   uint64_t* acc_full = empty + S;
   uint64_t* acc_free = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_free + 2);
+  uint64_t* old_full = acc_free + 2;
+  uint64_t* staging_free = old_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staging_free + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = G == 2 ? cluster_rank() : 0;
-  const long long first = (long long)blockIdx.x / G, step = gridDim.x / G;
-  const int k_blocks = (s.k + C::kKStage - 1) / C::kKStage;
+  const uint32_t cta = kCluster > 1 ? cluster_rank() : 0, rank = G == 2 ? cta : 0;
+  const int first = blockIdx.x / kCluster, step = gridDim.x / kCluster;
+  // the range of k blocks of this CTA (with an empty sum, one block of zeros)
+  const int all_blocks = max(1, (s.k + C::kKStage - 1) / C::kKStage);
+  const int kb_begin = C::SPLIT == 1 ? 0 : (int)(all_blocks * cta / C::SPLIT);
+  const int k_blocks = C::SPLIT == 1 ? all_blocks : (int)(all_blocks * (cta + 1) / C::SPLIT) - kb_begin;
 
   if (warp == 0 && lane == 0) {
+    if constexpr (!C::PLAIN) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    }
     for (int i = 0; i < S; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], C::PLAIN ? 8 : 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_free[i], 8 * G);
     }
+    mbar_init(old_full, 1);
+    mbar_init(staging_free, 1);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -126,7 +213,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     tc_fence_before();
   }
   __syncthreads();
-  if constexpr (G == 2) cluster_sync();
+  if constexpr (kCluster > 1) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // Everything above may overlap the end of the kernel before this one; its results are read from here on.
@@ -134,14 +221,28 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (lane == 0 && !C::PLAIN) {
       bool ok = true;
+      uint32_t tiles_done = 0;
+      const uint32_t cta_in_split = C::SPLIT > 1 ? cta : 0;
       uint32_t round = 0;
       int slot = 0;
-      for (long long t = first; t < s.tiles && ok; t += step) {
+      for (int t = first; t < s.tiles && ok; t += step) {
         const UmmaTile tile = umma_tile<C::kRatio>(s, t);
         const int za = (s.a_items == 1 ? 0 : tile.item) * C::PLANES, zb = (s.b_items == 1 ? 0 : tile.item) * C::PLANES;
         const int m0 = tile.tm * C::kBM + (int)rank * 128, n0 = tile.tn * C::BN + (int)rank * C::kBRows;
+        if constexpr (Epilogue::kStaged) {
+          if (ep.has_old) {
+            ok = mbar_wait(staging_free, (uint32_t)(tiles_done & 1) ^ 1, wait_code + kUmmaWaitStaging);
+            if (!ok) break;
+            constexpr int kOwn = C::BN / C::SPLIT;  // the columns that this CTA stores
+            mbar_arrive_expect_tx(old_full, C::PLANES * kOwn * 256);
+            for (int pl = 0; pl < C::PLANES; ++pl)
+              for (int c = 0; c < kOwn; c += kStagedColumns)
+                tma_load_3d(staging + (pl * kOwn + c) * 256, &map_old, m0, tile.tn * C::BN + (int)cta_in_split * kOwn + c, tile.item * C::PLANES + pl, old_full);
+          }
+          ++tiles_done;
+        }
         for (int kb = 0; kb < k_blocks && ok; ++kb) {
           ok = G == 1 ? mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty)
                       : mbar_wait_cluster(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty);
@@ -153,7 +254,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             if constexpr (G == 2) tma_load_3d_pair(smem_u32(dst), map, x, y, z, bar);
             else tma_load_3d(dst, map, x, y, z, &full[slot]);
           };
-          const int k0 = kb * C::kKStage;
+          const int k0 = (kb_begin + kb) * C::kKStage;
 #pragma unroll
           for (int pl = 0; pl < C::PLANES; ++pl) {
             unsigned char* a = stage + pl * C::kABytes;
@@ -205,8 +306,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       bool ok = true;
       uint32_t round = 0;
       int slot = 0;
-      long long done = 0;
-      for (long long t = first; t < s.tiles && ok; t += step) {
+      uint32_t done = 0;
+      for (int t = first; t < s.tiles && ok; t += step) {
         uint32_t d = 0;
         for (int kb = 0; kb < k_blocks; ++kb) {
           const bool begins = C::kChunk ? kb % (C::kChunk ? C::kChunk : 1) == 0 : kb == 0;
@@ -249,19 +350,18 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
     }
   } else {
-    // Two warps per quarter of the 128 rows: each takes half of the columns (narrow tiles: the first takes all).
-    constexpr int kSplit = C::BN >= 64 ? 2 : 1, kCols = C::BN / kSplit, kPiece = kCols < 32 ? 16 : 32;
+    // Two warps per quarter of the 128 rows: each takes half of the columns.
+    constexpr int kCols = C::BN / 2, kOwn = C::BN / C::SPLIT, kMine = kOwn / 2, W = kMine < 16 ? kMine : 16;
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + half * kCols;
-    long long done = 0;
+    uint32_t done = 0, tiles_done = 0;
     auto acquire = [&]() {
       const int acc = (int)(done & 1);
-      const bool ok = G == 1 ? mbar_wait(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc)
-                             : mbar_wait_cluster(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc);
-      if (!__all_sync(0xffffffffu, ok)) return false;
+      const bool got = G == 1 ? mbar_wait(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc)
+                              : mbar_wait_cluster(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc);
       tc_fence_after();
-      return true;
+      return (bool)__all_sync(0xffffffffu, got);
     };
     auto release = [&]() {
       tc_fence_before();
@@ -272,51 +372,173 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
       ++done;
     };
-    bool ok = true;
-    for (long long t = first; t < s.tiles && ok; t += step) {
+    bool ok = true, fetched = true;
+    uint32_t round = 0;
+    int slot = 0;
+    for (int t = first; t < s.tiles && ok; t += step) {
       const UmmaTile tile = umma_tile<C::kRatio>(s, t);
-      const int n0 = tile.tn * C::BN + half * kCols;
-      Epilogue epi(ep, s, tile, s.symmetric && tile.tn < C::kRatio * tile.tm, tile.tm * C::kBM + (int)rank * 128 + row);
-      if constexpr (C::kChunk == 0) {
-        ok = acquire();
-        if (!ok) break;
-        if (half < kSplit) {
-#pragma unroll 1
-          for (int c = 0; c < kCols; c += kPiece) {
-            if (n0 + c >= s.n) break;
-            uint32_t v[kPiece];
-            tmem_ld(v, lanes + (uint32_t)(done & 1) * C::BN + c);
-            tmem_wait_ld();
-            epi.store(v, n0 + c);
+      if constexpr (C::PLAIN) {
+        const int8_t* a = po.a + tile.item * po.sa;
+        const int8_t* b = po.b + tile.item * po.sb;
+        const int8_t* a_end = a + (long long)(s.m - 1) * po.lda + s.k;
+        const int8_t* b_end = b + (long long)(s.n - 1) * po.ldb + s.k;
+        const int tid = (int)threadIdx.x - 64;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty));
+          if (!ok) break;
+          unsigned char* stage = smem + (size_t)slot * C::kStageBytes;
+          const int chunk = tid & 7, kk = (kb_begin + kb) * 128 + chunk * 16, valid = s.k - kk;
+          constexpr int kRows = 128 + C::kBRows, kEach = kRows / 32;
+          Words16 v[kEach];
+          auto source = [&](int i, const int8_t*& at, const int8_t*& lo, const int8_t*& hi) {
+            const int r = (tid >> 3) + i * 32;
+            const bool is_a = r < 128;
+            const int index = is_a ? tile.tm * 128 + r : tile.tn * C::BN + r - 128;
+            lo = is_a ? a : b;
+            hi = is_a ? a_end : b_end;
+            at = lo + (long long)index * (is_a ? po.lda : po.ldb) + kk;
+            return index < (is_a ? s.m : s.n) && valid > 0;
+          };
+          const int8_t *at, *lo, *hi;
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) {
+            v[i] = Words16{make_uint4(0, 0, 0, 0), false};
+            if (source(i, at, lo, hi)) v[i] = load16_words(at, valid, lo, hi);
           }
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) {
+            const int r = (tid >> 3) + i * 32;  // the rows of A, then those of B: both start on a multiple of eight rows
+            if (v[i].edge && source(i, at, lo, hi)) v[i].v = load16_bytes(at, valid);
+            *reinterpret_cast<uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4)) = v[i].v;
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[slot]);
+          if (++slot == S) {
+            slot = 0;
+            ++round;
+          }
+        }
+        fetched = ok;
+      }
+      const int m = tile.tm * C::kBM + (int)rank * 128 + row;
+      const int mine = tile.tn * C::BN + (C::SPLIT > 1 ? (int)cta * kOwn : 0) + half * kMine;  // first of this thread's columns
+      const bool twice = s.symmetric && tile.tn < C::kRatio * tile.tm;
+      typename Epilogue::template Tile<W> epi(ep, s, tile, twice, m, mine, staging + half * kMine * 256 + row * 2, kOwn * 256);
+      if constexpr (C::kChunk == 0) {
+        ok = k_blocks == 0 || acquire();
+      } else if (k_blocks > 0) {
+        // the chunks' sums, rounded to nearest, go back to where the last chunk was
+        uint32_t v[kCols / 32][32] = {};
+        for (int kb = 0; kb < k_blocks && ok; kb += C::kChunk) {
+          ok = acquire();
+#pragma unroll
+          for (int c = 0; c < kCols / 32; ++c) {
+            uint32_t w[32];
+            tmem_ld(w, lanes + (uint32_t)(done & 1) * C::BN + c * 32);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[c][i] = __float_as_uint(__uint_as_float(v[c][i]) + __uint_as_float(w[i]));
+          }
+          if (kb + C::kChunk < k_blocks) release();
+        }
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) tmem_st(lanes + (uint32_t)(done & 1) * C::BN + c * 32, v[c]);
+        tmem_wait_st();
+      }
+      if constexpr (Epilogue::kStaged) {
+        const uint32_t parity = (uint32_t)(tiles_done & 1);
+        if (ep.has_old) ok = mbar_wait(old_full, parity, wait_code + kUmmaWaitOld) && ok;
+        else ok = mbar_wait(staging_free, parity ^ 1, wait_code + kUmmaWaitStaging) && ok;
+        ++tiles_done;
+      }
+      ok = named_all(ok && fetched, 256);
+      __syncwarp();
+      if constexpr (C::SPLIT == 1) {
+        if (!ok) break;
+#pragma unroll 1
+        for (int c = 0; c < kMine; c += W) {
+          if (mine + c >= s.n) break;
+          uint32_t v[W];
+          tmem_ld(v, lanes + (uint32_t)(done & 1) * C::BN + c);
+          tmem_wait_ld();
+          epi.group(v, c);
         }
         release();
       } else {
-        uint32_t v[kCols / kPiece][kPiece] = {};
-        for (int kb = 0; kb < k_blocks; kb += C::kChunk) {
-          ok = acquire();
-          if (!ok) break;
-#pragma unroll
-          for (int c = 0; c < kCols / kPiece; ++c) {
-            uint32_t w[kPiece];
-            tmem_ld(w, lanes + (uint32_t)(done & 1) * C::BN + c * kPiece);
+        // The cluster has this one tile.  Once every CTA is past its products the stages are free: column c goes to the CTA
+        // c / kOwn, into its slab for this CTA.
+        cluster_sync();
+#pragma unroll 1
+        for (int c = 0; c < kCols; c += 16) {
+          uint32_t v[16] = {};
+          if (k_blocks > 0) {
+            tmem_ld(v, lanes + (uint32_t)(done & 1) * C::BN + c);
             tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < kPiece; ++i)
-              v[c][i] = __float_as_uint(__uint_as_float(v[c][i]) + __uint_as_float(w[i]));
           }
-          release();
-        }
-        if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < kCols / kPiece; ++c)
-          if (n0 + c * kPiece < s.n) epi.store(v[c], n0 + c * kPiece);
+          for (int i = 0; i < 16; ++i) {
+            const int col = half * kCols + c + i;
+            const uint32_t to = cluster_addr(smem_u32(smem), col / kOwn) + ((cta * kOwn + col % kOwn) * 128 + row) * 4;
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(v[i]) : "memory");
+          }
+        }
+        cluster_sync();
+        if (!ok) break;
+        const uint32_t* sums = reinterpret_cast<const uint32_t*>(smem);
+#pragma unroll 1
+        for (int c = 0; c < kMine; c += W) {
+          if (mine + c >= s.n) break;
+          uint32_t v[W];
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const int col = half * kMine + c + i;
+            v[i] = sums[col * 128 + row];
+#pragma unroll
+            for (int from = 1; from < C::SPLIT; ++from) {
+              const uint32_t w = sums[(from * kOwn + col) * 128 + row];
+              v[i] = C::I8 ? v[i] + w : __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(w));
+            }
+          }
+          epi.group(v, c);
+        }
       }
+      if constexpr (Epilogue::kStaged) {
+        fence_async_smem();
+        named_all(true, 256);
+        if (threadIdx.x == 64) {
+          if constexpr (Epilogue::kStagedOut) {
+            const int first_col = tile.tn * C::BN + (C::SPLIT > 1 ? (int)cta * kOwn : 0);
+            for (int pl = 0; pl < C::PLANES; ++pl)
+              for (int c = 0; c < kOwn; c += kStagedColumns)
+                if (first_col + c < s.n && tile.tm * C::kBM + (int)rank * 128 < s.m)
+                  tma_store_3d(&map_out, staging + (pl * kOwn + c) * 256, tile.tm * C::kBM + (int)rank * 128, first_col + c, tile.item * C::PLANES + pl);
+            bulk_commit();
+            bulk_wait_read<0>();
+          }
+          mbar_arrive(staging_free);
+        }
+      }
+    }
+    // as the producer does
+    for (int i = 0; i < S && C::PLAIN && ok && fetched; ++i) {
+      ok = mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty);
+      if (++slot == S) {
+        slot = 0;
+        ++round;
+      }
+    }
+  }
+  if constexpr (C::SPLIT > 1) {
+    if (warp < 2) {  // the two exchanges of the epilogue warps
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
     }
   }
   __syncwarp();
   __syncthreads();
-  if constexpr (G == 2) cluster_sync();
+  if constexpr (kCluster > 1) cluster_sync();
   if (warp == 1) {
     tc_fence_after();
     tmem_free<G>(tmem, C::kTmemColumns);
@@ -324,51 +546,57 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 }
 
 // ---- host side -----------------------------------------------------------------------------------
-// 3-D map (inner, outer, z) over `base`: box of 128 bytes x box_outer rows x 1, 128-byte swizzle.  Strides in bytes.
+// 3-D map (inner, outer, z) over `base`: box of 128 bytes x box_outer rows x 1, 128-byte swizzle; `staged` (half only): box of 128
+// elements x box_outer rows without a swizzle, for the staging buffer.  Strides in bytes.
 inline int encode_operand(CUtensorMap* map, const void* base, bool i8, long long inner, long long outer, long long z, long long ld_bytes,
-                          long long z_bytes, int box_outer) {
+                          long long z_bytes, int box_outer, bool staged = false) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return BLB200_E_INTERNAL;
   const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)z};
   const cuuint64_t strides[2] = {(cuuint64_t)ld_bytes, (cuuint64_t)(z > 1 ? z_bytes : ld_bytes * outer)};
-  const cuuint32_t box[3] = {i8 ? 128u : 64u, (cuuint32_t)box_outer, 1}, estr[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {i8 || staged ? 128u : 64u, (cuuint32_t)box_outer, 1}, estr[3] = {1, 1, 1};
   const CUresult r = enc(map, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides,
-                         box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, staged ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? BLB200_OK : BLB200_E_INTERNAL;
 }
 
 template <class C, class Epilogue>
-int launch_umma(const CUtensorMap& map_a, const CUtensorMap& map_b, UmmaShape s, const typename Epilogue::Params& ep, int wait_code,
-                cudaStream_t stream) {
+int launch_umma(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_old, const CUtensorMap& map_out, UmmaShape s, const typename Epilogue::Params& ep, int wait_code,
+                cudaStream_t stream, const PlainOperands& po = PlainOperands{}) {
+  constexpr int kCluster = C::GROUP * C::SPLIT;
   s.tiles_m = (s.m + C::kBM - 1) / C::kBM;
   s.tiles_n = (s.n + C::BN - 1) / C::BN;
-  s.tiles = (s.symmetric ? symmetric_tiles<C::kRatio>(s.tiles_m, s.tiles_n) : (long long)s.tiles_m * s.tiles_n) * s.batch;
+  const long long tiles = (s.symmetric ? (long long)symmetric_tiles<C::kRatio>(s.tiles_m, s.tiles_n) : (long long)s.tiles_m * s.tiles_n) * s.batch;
+  if (tiles > 0x3fffffffll || (long long)s.tiles_m * s.tiles_n > 0x3fffffffll) return BLB200_E_TOO_LARGE;
+  s.tiles = (int)tiles;
   auto kern = umma_gemm_kernel<C, Epilogue>;
   static thread_local int configured_for = -1;
   int cur = 0;
   cudaGetDevice(&cur);
   if (configured_for != cur) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)UmmaMemory<C, Epilogue>::kBytes);
     if (e != cudaSuccess) return (int)e;
     configured_for = cur;
   }
-  const long long units = device_info().sm_count / C::GROUP;
+  // a split tile has a cluster of its own, otherwise the CTAs or pairs that the device holds walk over the tiles
+  const long long units = C::SPLIT > 1 ? s.tiles : device_info().sm_count / C::GROUP;
+  if (units * kCluster > 0x7fffffffll) return BLB200_E_TOO_LARGE;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((s.tiles < units ? s.tiles : units) * C::GROUP));
+  cfg.gridDim = dim3((unsigned)((s.tiles < units ? s.tiles : units) * kCluster));
   cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.dynamicSmemBytes = UmmaMemory<C, Epilogue>::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = C::GROUP;
+  attr[1].val.clusterDim.x = kCluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = C::GROUP == 2 ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_b, s, ep, wait_code);
+  cfg.numAttrs = kCluster > 1 ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_b, map_old, map_out, s, ep, po, wait_code);
 }
 
 }  // namespace blb200
