@@ -124,7 +124,7 @@ struct PlainOperands {
   long long lda, ldb, sa, sb;
 };
 
-// 16 bytes at `src` (any alignment) of which the first `valid` (at least 1) exist, the rest zero.  [lo, hi) is the operand: aligned
+// 16 bytes at `src` (any alignment) of which the first `valid` exist, the rest zero.  [lo, hi) is the operand: aligned
 // words that lie inside it are read whole and shifted together, without branches, so that many such loads can be in flight;
 // `edge` says that a word reaches over one of its ends, and load16_bytes has to do it.
 struct Words16 {
@@ -223,26 +223,12 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   if (warp == 0) {
     if (lane == 0 && !C::PLAIN) {
       bool ok = true;
-      uint32_t tiles_done = 0;
-      const uint32_t cta_in_split = C::SPLIT > 1 ? cta : 0;
       uint32_t round = 0;
       int slot = 0;
       for (int t = first; t < s.tiles && ok; t += step) {
         const UmmaTile tile = umma_tile<C::kRatio>(s, t);
         const int za = (s.a_items == 1 ? 0 : tile.item) * C::PLANES, zb = (s.b_items == 1 ? 0 : tile.item) * C::PLANES;
         const int m0 = tile.tm * C::kBM + (int)rank * 128, n0 = tile.tn * C::BN + (int)rank * C::kBRows;
-        if constexpr (Epilogue::kStaged) {
-          if (ep.has_old) {
-            ok = mbar_wait(staging_free, (uint32_t)(tiles_done & 1) ^ 1, wait_code + kUmmaWaitStaging);
-            if (!ok) break;
-            constexpr int kOwn = C::BN / C::SPLIT;  // the columns that this CTA stores
-            mbar_arrive_expect_tx(old_full, C::PLANES * kOwn * 256);
-            for (int pl = 0; pl < C::PLANES; ++pl)
-              for (int c = 0; c < kOwn; c += kStagedColumns)
-                tma_load_3d(staging + (pl * kOwn + c) * 256, &map_old, m0, tile.tn * C::BN + (int)cta_in_split * kOwn + c, tile.item * C::PLANES + pl, old_full);
-          }
-          ++tiles_done;
-        }
         for (int kb = 0; kb < k_blocks && ok; ++kb) {
           ok = G == 1 ? mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty)
                       : mbar_wait_cluster(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty);
@@ -372,6 +358,18 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
       ++done;
     };
+    // The staging buffer's owner sends for a tile's old values as soon as the tile before has left it.
+    auto request_old = [&](int t) {
+      const UmmaTile tile = umma_tile<C::kRatio>(s, t);
+      mbar_arrive_expect_tx(old_full, C::PLANES * kOwn * 256);
+      for (int pl = 0; pl < C::PLANES; ++pl)
+        for (int c = 0; c < kOwn; c += kStagedColumns)
+          tma_load_3d(staging + (pl * kOwn + c) * 256, &map_old, tile.tm * C::kBM + (int)rank * 128,
+                      tile.tn * C::BN + (C::SPLIT > 1 ? (int)cta * kOwn : 0) + c, tile.item * C::PLANES + pl, old_full);
+    };
+    if constexpr (Epilogue::kStaged) {
+      if (threadIdx.x == 64 && ep.has_old && first < s.tiles) request_old(first);
+    }
     bool ok = true, fetched = true;
     uint32_t round = 0;
     int slot = 0;
@@ -394,22 +392,33 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             const int r = (tid >> 3) + i * 32;
             const bool is_a = r < 128;
             const int index = is_a ? tile.tm * 128 + r : tile.tn * C::BN + r - 128;
+            const bool exists = index < (is_a ? s.m : s.n) && valid > 0;
             lo = is_a ? a : b;
             hi = is_a ? a_end : b_end;
-            at = lo + (long long)index * (is_a ? po.lda : po.ldb) + kk;
-            return index < (is_a ? s.m : s.n) && valid > 0;
+            at = exists ? lo + (long long)index * (is_a ? po.lda : po.ldb) + kk : lo;
+            return exists ? valid : 0;
           };
           const int8_t *at, *lo, *hi;
 #pragma unroll
           for (int i = 0; i < kEach; ++i) {
-            v[i] = Words16{make_uint4(0, 0, 0, 0), false};
-            if (source(i, at, lo, hi)) v[i] = load16_words(at, valid, lo, hi);
+            const int bytes = source(i, at, lo, hi);
+            v[i] = load16_words(at, bytes, lo, hi);
           }
+          bool edge = false;
 #pragma unroll
-          for (int i = 0; i < kEach; ++i) {
-            const int r = (tid >> 3) + i * 32;  // the rows of A, then those of B: both start on a multiple of eight rows
-            if (v[i].edge && source(i, at, lo, hi)) v[i].v = load16_bytes(at, valid);
-            *reinterpret_cast<uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4)) = v[i].v;
+          for (int i = 0; i < kEach; ++i) edge |= v[i].edge;
+          if (edge) {
+#pragma unroll 1
+            for (int i = 0; i < kEach; ++i) {
+              const int bytes = source(i, at, lo, hi), r = (tid >> 3) + i * 32;
+              *reinterpret_cast<uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4)) = load16_bytes(at, bytes);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+              const int r = (tid >> 3) + i * 32;  // the rows of A, then those of B: both start on a multiple of eight rows
+              *reinterpret_cast<uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4)) = v[i].v;
+            }
           }
           fence_async_smem();
           __syncwarp();
@@ -516,7 +525,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             bulk_commit();
             bulk_wait_read<0>();
           }
-          mbar_arrive(staging_free);
+          if (!ep.has_old) mbar_arrive(staging_free);
+          else if (t + step < s.tiles) request_old(t + step);
         }
       }
     }
