@@ -22,10 +22,10 @@ struct GemmI8Params {
   float alpha, beta;
 };
 
-// alpha * (acc * sa) * sb + beta * prior, in float, rounded once to T.
+// acc * (alpha sa) * sb + beta * prior, in float, rounded once to T.
 template <typename T>
 __device__ __forceinline__ void store_c(T* c, int acc, float sa, float sb, float alpha, float beta) {
-  float v = alpha * (((float)acc * sa) * sb);
+  float v = (float)acc * (sa * alpha) * sb;
   if (beta != 0.f) v = fmaf(beta, to_f32(*c), v);
   *c = from_f32<T>(v);
 }
@@ -53,7 +53,7 @@ __device__ __forceinline__ uint4 load16(const int8_t* src, int valid, const int8
   if (WHOLE && valid >= 16) return *reinterpret_cast<const uint4*>(src);
   if (valid <= 0) return make_uint4(0, 0, 0, 0);
   const Words16 w = load16_words(src, valid, lo, hi);
-  return w.edge ? load16_bytes(src, valid) : w.v;
+  return w.edge ? load16_bytes(src, valid) : valid < 16 ? first_bytes(w.v, valid) : w.v;
 }
 
 // WHOLE: both operands' columns start on 16-byte boundaries.
@@ -180,38 +180,64 @@ struct I8Params {
   int ftype;
 };
 
+// The scales of a warp's columns are brought into shared memory while the products run; a whole group of columns with beta = 0
+// then costs about seven instructions per column and row of 32 (with the scale read from memory, the bounds and beta
+// tested for each element it was 36, and the epilogue, not the MMAs, set the time of an 8192^3 product).
 struct I8Epilogue {
   using Params = I8Params;
   static constexpr bool kStaged = false;
-  template <int W>
+  static constexpr int kWarpBytesPerColumn = 4;
+  template <int W, int COLS>
   struct Tile;
 };
-template <int W>
+template <int W, int COLS>
 struct I8Epilogue::Tile {
   const I8Params& p;
+  float* scales;
   long long item, m;
   int n0;
   float sa;
   bool live;
-  __device__ Tile(const Params& p_, const UmmaShape&, const UmmaTile& tile, bool, int m_, int n, unsigned char*, int)
-      : p(p_), item(tile.item), m(m_), n0(n), live(m_ < p_.g.m) {
+  __device__ __forceinline__ Tile(const Params& p_, const UmmaShape&, const UmmaTile& tile, bool, int m_, int n, unsigned char* scratch, int)
+      : p(p_), scales(reinterpret_cast<float*>(scratch)), item(tile.item), m(m_), n0(n), live(m_ < p_.g.m) {
     sa = p.g.scale_a && live ? p.g.scale_a[item * p.g.ssa + m] : 1.f;
+    sa *= p.g.alpha;
+    const float* sb = p.g.scale_b ? p.g.scale_b + item * p.g.ssb + n : nullptr;
+    __syncwarp();
+    for (int i = threadIdx.x & 31; i < COLS; i += 32) scales[i] = sb && n + i < p.g.n ? sb[i] : 1.f;
+    __syncwarp();
   }
   // Columns n0 + c ... n0 + c + W - 1 of the row.
   __device__ __forceinline__ void group(const uint32_t (&v)[W], int c) {
-    const int n = n0 + c;
-    if (!live || n >= p.g.n) return;
-    if (p.ftype == BLB200_F32) store_as<float>(v, n);
-    else if (p.ftype == BLB200_F16) store_as<__half>(v, n);
-    else store_as<__nv_bfloat16>(v, n);
+    if (!live) return;
+    if (p.ftype == BLB200_F32) store_as<float>(v, c);
+    else if (p.ftype == BLB200_F16) store_as<__half>(v, c);
+    else store_as<__nv_bfloat16>(v, c);
   }
   template <typename T>
-  __device__ __forceinline__ void store_as(const uint32_t (&v)[W], int n) {
+  __device__ __forceinline__ void store_as(const uint32_t (&v)[W], int c) {
+    const int n = n0 + c;
     T* at = (T*)p.g.c + item * p.g.sc + m + (long long)n * p.g.ldc;
-    const float* sb = p.g.scale_b ? p.g.scale_b + item * p.g.ssb + n : nullptr;
+    float r[W];
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const float4 sb = *reinterpret_cast<const float4*>(scales + c + i);
+      r[i] = (float)(int)v[i] * sa * sb.x;
+      r[i + 1] = (float)(int)v[i + 1] * sa * sb.y;
+      r[i + 2] = (float)(int)v[i + 2] * sa * sb.z;
+      r[i + 3] = (float)(int)v[i + 3] * sa * sb.w;
+    }
+    if (p.g.beta == 0.f && n + W <= p.g.n) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        *at = from_f32<T>(r[i]);
+        at += p.g.ldc;
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      if (n + i < p.g.n) store_c(at, (int)v[i], sa, sb ? sb[i] : 1.f, p.g.alpha, p.g.beta);
+      if (n + i < p.g.n) *at = from_f32<T>(p.g.beta != 0.f ? fmaf(p.g.beta, to_f32(*at), r[i]) : r[i]);
       at += p.g.ldc;
     }
   }

@@ -127,8 +127,9 @@ struct NsEpilogue {
     long long out_ld, out_plane, out_item;
   };
   static constexpr bool kStaged = true, kStagedOut = !LAST;
+  static constexpr int kWarpBytesPerColumn = 0;
   // One thread's row of a tile, from column n0 on; `staged` is its element of column n0 in the staging buffer.
-  template <int W>
+  template <int W, int COLS>
   struct Tile {
     const Params& p;
     const UmmaShape& s;

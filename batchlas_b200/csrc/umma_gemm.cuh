@@ -72,7 +72,8 @@ struct UmmaConfig {
 // Shared memory of one kernel: the ring, the exchange area of the epilogue, the barriers.
 template <class C, class Epilogue>
 struct UmmaMemory {
-  static constexpr int kStaging = Epilogue::kStaged ? C::PLANES * C::BN * 256 : 0;
+  // half columns of the result's tile, or what the epilogue's eight warps keep for themselves
+  static constexpr int kStaging = Epilogue::kStaged ? C::PLANES * C::BN * 256 : C::BN / 2 * Epilogue::kWarpBytesPerColumn * 8;
   static constexpr int kFit = (224 * 1024 - kStaging) / C::kStageBytes;
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr size_t kBytes = 1024 + kStaging + (size_t)kStages * C::kStageBytes + 256;
@@ -124,9 +125,9 @@ struct PlainOperands {
   long long lda, ldb, sa, sb;
 };
 
-// 16 bytes at `src` (any alignment) of which the first `valid` exist, the rest zero.  [lo, hi) is the operand: aligned
-// words that lie inside it are read whole and shifted together, without branches, so that many such loads can be in flight;
-// `edge` says that a word reaches over one of its ends, and load16_bytes has to do it.
+// 16 bytes at `src` (any alignment) of which the first `valid` exist, the rest zero.  [lo, hi) is the operand.  The five aligned
+// words around them are read and shifted together, without branches, so that many such loads can be in flight; where
+// one of them reaches over an end of the operand, `edge` says so and load16_bytes has to do it.
 struct Words16 {
   uint4 v;
   bool edge;
@@ -134,23 +135,20 @@ struct Words16 {
 __device__ __forceinline__ Words16 load16_words(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
   const int off = (int)(reinterpret_cast<uintptr_t>(src) & 3u);
   const int8_t* base = src - off;
+  const bool exists = valid > 0, inside = base >= lo && base + 20 <= hi;
   uint32_t x[5];
-  bool edge = false;
 #pragma unroll
   for (int j = 0; j < 5; ++j) {
-    const bool needed = 4 * j - off < min(valid, 16), inside = base + 4 * j >= lo && base + 4 * j + 4 <= hi;
     x[j] = 0;
-    if (needed && inside) x[j] = *reinterpret_cast<const uint32_t*>(base + 4 * j);
-    edge |= needed && !inside;
+    if (exists && inside) x[j] = reinterpret_cast<const uint32_t*>(base)[j];
   }
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    w[j] = __funnelshift_r(x[j], x[j + 1], off * 8);
-    const int left = valid - 4 * j;
-    if (left < 4) w[j] &= left > 0 ? 0xffffffffu >> (8 * (4 - left)) : 0u;
-  }
-  return Words16{make_uint4(w[0], w[1], w[2], w[3]), edge};
+  return Words16{make_uint4(__funnelshift_r(x[0], x[1], off * 8), __funnelshift_r(x[1], x[2], off * 8), __funnelshift_r(x[2], x[3], off * 8),
+                            __funnelshift_r(x[3], x[4], off * 8)),
+                 exists && !inside};
+}
+__device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >= 4 ? w : n <= 0 ? 0u : w & (0xffffffffu >> (8 * (4 - n))); }
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
+  return make_uint4(first_bytes(v.x, n), first_bytes(v.y, n - 4), first_bytes(v.z, n - 8), first_bytes(v.w, n - 12));
 }
 static __device__ __noinline__ uint4 load16_bytes(const int8_t* src, int valid) {
   uint32_t w[4] = {0, 0, 0, 0};
@@ -387,38 +385,29 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           unsigned char* stage = smem + (size_t)slot * C::kStageBytes;
           const int chunk = tid & 7, kk = (kb_begin + kb) * 128 + chunk * 16, valid = s.k - kk;
           constexpr int kRows = 128 + C::kBRows, kEach = kRows / 32;
+          // rows (tid >> 3) + 32 i: those of A (i < 4), then those of B; both start on a multiple of eight rows
+          const int r0 = tid >> 3, ma = tile.tm * 128 + r0, nb = tile.tn * C::BN + r0;
+          const int8_t* at_a = a + (long long)ma * po.lda + kk;
+          const int8_t* at_b = b + (long long)nb * po.ldb + kk;
+          unsigned char* to = stage + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
+          auto bytes_of = [&](int i) { return (i < 4 ? ma + 32 * i < s.m : nb + 32 * (i - 4) < s.n) ? valid : 0; };
+          auto source = [&](int i) { return i < 4 ? at_a + (long long)(32 * i) * po.lda : at_b + (long long)(32 * (i - 4)) * po.ldb; };
           Words16 v[kEach];
-          auto source = [&](int i, const int8_t*& at, const int8_t*& lo, const int8_t*& hi) {
-            const int r = (tid >> 3) + i * 32;
-            const bool is_a = r < 128;
-            const int index = is_a ? tile.tm * 128 + r : tile.tn * C::BN + r - 128;
-            const bool exists = index < (is_a ? s.m : s.n) && valid > 0;
-            lo = is_a ? a : b;
-            hi = is_a ? a_end : b_end;
-            at = exists ? lo + (long long)index * (is_a ? po.lda : po.ldb) + kk : lo;
-            return exists ? valid : 0;
-          };
-          const int8_t *at, *lo, *hi;
-#pragma unroll
-          for (int i = 0; i < kEach; ++i) {
-            const int bytes = source(i, at, lo, hi);
-            v[i] = load16_words(at, bytes, lo, hi);
-          }
           bool edge = false;
 #pragma unroll
-          for (int i = 0; i < kEach; ++i) edge |= v[i].edge;
+          for (int i = 0; i < kEach; ++i) {
+            v[i] = load16_words(source(i), bytes_of(i), i < 4 ? a : b, i < 4 ? a_end : b_end);
+            edge |= v[i].edge;
+          }
+          if (valid < 16) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) v[i].v = first_bytes(v[i].v, valid);
+          }
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) *reinterpret_cast<uint4*>(to + i * 32 * 128) = v[i].v;
           if (edge) {
 #pragma unroll 1
-            for (int i = 0; i < kEach; ++i) {
-              const int bytes = source(i, at, lo, hi), r = (tid >> 3) + i * 32;
-              *reinterpret_cast<uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4)) = load16_bytes(at, bytes);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-              const int r = (tid >> 3) + i * 32;  // the rows of A, then those of B: both start on a multiple of eight rows
-              *reinterpret_cast<uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4)) = v[i].v;
-            }
+            for (int i = 0; i < kEach; ++i) *reinterpret_cast<uint4*>(to + i * 32 * 128) = load16_bytes(source(i), bytes_of(i));
           }
           fence_async_smem();
           __syncwarp();
@@ -433,7 +422,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       const int m = tile.tm * C::kBM + (int)rank * 128 + row;
       const int mine = tile.tn * C::BN + (C::SPLIT > 1 ? (int)cta * kOwn : 0) + half * kMine;  // first of this thread's columns
       const bool twice = s.symmetric && tile.tn < C::kRatio * tile.tm;
-      typename Epilogue::template Tile<W> epi(ep, s, tile, twice, m, mine, staging + half * kMine * 256 + row * 2, kOwn * 256);
+      unsigned char* scratch = Epilogue::kStaged ? staging + half * kMine * 256 + row * 2 : staging + (warp - 2) * (M::kStaging / 8);
+      typename Epilogue::template Tile<W, kMine> epi(ep, s, tile, twice, m, mine, scratch, kOwn * 256);
       if constexpr (C::kChunk == 0) {
         ok = k_blocks == 0 || acquire();
       } else if (k_blocks > 0) {
