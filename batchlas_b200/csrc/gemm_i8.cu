@@ -250,23 +250,28 @@ struct TileChoice {
   int group, bn, split;
   double time;
 };
-double tile_time(const GemmI8Params& p, int group, int bn, int split) {
-  const long long sms = device_info().sm_count, bm = 128 * group;
-  const long long tiles = (p.m + bm - 1) / bm * ((p.n + bn - 1) / bn) * p.batch;
-  const double blocks = (double)((p.k + 127) / 128), per = std::max(2.0 * bn, (16384.0 + 128.0 * bn / group) / 50.0);
-  if (split > 1 && tiles * split > sms) return 1e300;
-  const double rounds = split > 1 ? 1.0 : (double)((tiles + sms / group - 1) / (sms / group));
-  return rounds * (ceil(blocks / split) * per + 2500.0) + (split > 1 ? 1500.0 : 0.0);
+template <int GROUP, int BN, int SPLIT, bool PLAIN>
+double tile_time(const GemmI8Params& p) {
+  constexpr int kBM = 128 * GROUP;
+  const long long units = umma_capacity<UmmaConfig<true, false, false, GROUP, BN, 1, SPLIT, PLAIN>, I8Epilogue>();
+  const long long tiles = (long long)((p.m + kBM - 1) / kBM) * ((p.n + BN - 1) / BN) * p.batch;
+  if (SPLIT > 1 && tiles > units) return 1e300;
+  const double blocks = (double)((p.k + 127) / 128), per = std::max(2.0 * BN, (16384.0 + 128.0 * BN / GROUP) / 50.0);
+  return (double)((tiles + units - 1) / units) * (ceil(blocks / SPLIT) * per + 2500.0) + (SPLIT > 1 ? 1500.0 : 0.0);
 }
-TileChoice choose_tiles(const GemmI8Params& p, bool aligned) {
-  TileChoice best{1, 128, 1, tile_time(p, 1, 128, 1)};
-  auto consider = [&](int group, int bn, int split) {
-    const double t = tile_time(p, group, bn, split);
+template <bool PLAIN>
+TileChoice choose_tiles(const GemmI8Params& p) {
+  TileChoice best{1, 128, 1, tile_time<1, 128, 1, PLAIN>(p)};
+  auto consider = [&](int group, int bn, int split, double t) {
     if (t < best.time) best = TileChoice{group, bn, split, t};
   };
-  for (int bn : {64, 128})
-    for (int split : {1, 2, 4, 8}) consider(1, bn, split);
-  if (aligned) consider(2, 256, 1);
+  consider(1, 128, 2, tile_time<1, 128, 2, PLAIN>(p));
+  consider(1, 128, 4, tile_time<1, 128, 4, PLAIN>(p));
+  consider(1, 64, 1, tile_time<1, 64, 1, PLAIN>(p));
+  consider(1, 64, 2, tile_time<1, 64, 2, PLAIN>(p));
+  consider(1, 64, 4, tile_time<1, 64, 4, PLAIN>(p));
+  consider(1, 64, 8, tile_time<1, 64, 8, PLAIN>(p));
+  if constexpr (!PLAIN) consider(2, 256, 1, tile_time<2, 256, 1, false>(p));
   return best;
 }
 
@@ -301,7 +306,7 @@ int launch_tiles_i8(const GemmI8Params& p, const TileChoice& c, int ftype, cudaS
 #define BLB_TILE(BN_, SPLIT_) \
   if (c.bn == BN_ && c.split == SPLIT_) return launch_umma_i8<1, BN_, SPLIT_, PLAIN>(p, ftype, stream);
   BLB_TILE(64, 1) BLB_TILE(64, 2) BLB_TILE(64, 4) BLB_TILE(64, 8)
-  BLB_TILE(128, 1) BLB_TILE(128, 2) BLB_TILE(128, 4) BLB_TILE(128, 8)
+  BLB_TILE(128, 1) BLB_TILE(128, 2) BLB_TILE(128, 4)
 #undef BLB_TILE
   return BLB200_E_INTERNAL;
 }
@@ -310,10 +315,10 @@ int dispatch_gemm_i8(const GemmI8Params& p, int ftype, cudaStream_t stream) {
   if (p.n <= kFewColumns && ((long long)(p.m + 15) / 16) * p.batch <= 0x7fffffffll) return launch_gemm_i8_few(p, ftype, stream);
   const bool aligned = p.k > 0 && columns_16(p.a, p.lda, p.sa, p.m, p.batch) && columns_16(p.b, p.ldb, p.sb, p.n, p.batch);
   if (aligned) {
-    const int rc = launch_tiles_i8<false>(p, choose_tiles(p, true), ftype, stream);
+    const int rc = launch_tiles_i8<false>(p, choose_tiles<false>(p), ftype, stream);
     if (rc != BLB200_E_INTERNAL) return rc;  // a driver that refuses the tensor maps: plain loads take it
   }
-  return launch_tiles_i8<true>(p, choose_tiles(p, false), ftype, stream);
+  return launch_tiles_i8<true>(p, choose_tiles<true>(p), ftype, stream);
 }
 
 constexpr int kMaxK = 131071;  // 128 * 128 * k stays below 2^31

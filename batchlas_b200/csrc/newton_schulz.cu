@@ -281,10 +281,14 @@ int product(Maps& maps, const Operands& o, const typename Epilogue::Params& ep, 
   };
   const long long sms = device_info().sm_count, blocks = (o.k + 63) / 64;
   auto rounds = [](long long n, long long units) { return (double)((n + units - 1) / units); };
+  using Pair = UmmaConfig<false, A_MN, B_MN, 2, kPairN, PLANES>;
+  const long long pairs = umma_capacity<Pair, Epilogue>();
   const double block = PLANES == 2 ? 2.5 : 1.0, pair_block = PLANES == 2 ? 2.5 : 1.3;
-  const double pair = rounds(tiles(256, kPairN), sms / 2) * (blocks * pair_block + 12);
+  const double pair = rounds(tiles(256, kPairN), pairs) * (blocks * pair_block + 12);
   const double single = rounds(tiles(128, 128), sms) * (blocks * block + 12);
-  auto split = [&](int s) { return tiles(128, 128) * s > sms ? 1e300 : (double)((blocks + s - 1) / s) * block + 18; };
+  const long long most[2] = {umma_capacity<UmmaConfig<false, A_MN, B_MN, 1, 128, PLANES, 2>, Epilogue>(),
+                             umma_capacity<UmmaConfig<false, A_MN, B_MN, 1, 128, PLANES, 4>, Epilogue>()};
+  auto split = [&](int s) { return tiles(128, 128) > most[s / 4] ? 1e300 : (double)((blocks + s - 1) / s) * block + 18; };
   const double best = std::min(std::min(pair, single), std::min(split(2), split(4)));
   if (best == pair) return launch_product<A_MN, B_MN, 2, kPairN, PLANES, 1, Epilogue>(maps, o, ep, stream);
   if (best == single) return launch_product<A_MN, B_MN, 1, 128, PLANES, 1, Epilogue>(maps, o, ep, stream);
@@ -336,7 +340,7 @@ Layout layout_of(const blb200_newton_schulz_desc* d) {
     return here;
   };
   l.parts = take(n * kNormParts * sizeof(double));
-  l.factors = take(n * 3 * d->steps * sizeof(float2));
+  l.factors = take(n * 3 * kMaxSteps * sizeof(float2));
   l.x = take(n * l.planes * l.plane_x * 2);
   l.x2 = take(n * l.planes * l.plane_x * 2);
   l.s = take(n * l.planes * l.plane_s * 2);

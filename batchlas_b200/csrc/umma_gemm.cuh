@@ -31,6 +31,8 @@
 // copies still in flight are waited for, tensor memory is freed and the kernel returns.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -228,8 +230,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const int za = (s.a_items == 1 ? 0 : tile.item) * C::PLANES, zb = (s.b_items == 1 ? 0 : tile.item) * C::PLANES;
         const int m0 = tile.tm * C::kBM + (int)rank * 128, n0 = tile.tn * C::BN + (int)rank * C::kBRows;
         for (int kb = 0; kb < k_blocks && ok; ++kb) {
-          ok = G == 1 ? mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty)
-                      : mbar_wait_cluster(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty);
+          ok = mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty);
           if (!ok) break;
           if (rank == 0) mbar_arrive_expect_tx(&full[slot], G * C::kStageBytes);
           const uint32_t bar = G == 2 ? cluster_addr(smem_u32(&full[slot]), 0) : smem_u32(&full[slot]);
@@ -264,8 +265,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
       // No CTA leaves while MMA completions may still be signalled to its barriers.
       for (int i = 0; i < S && ok; ++i) {
-        ok = G == 1 ? mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty)
-                    : mbar_wait_cluster(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty);
+        ok = mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty);
         if (ok && ++slot == S) {
           slot = 0;
           ++round;
@@ -297,13 +297,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           const bool begins = C::kChunk ? kb % (C::kChunk ? C::kChunk : 1) == 0 : kb == 0;
           if (begins) {
             const int acc = (int)(done & 1);
-            ok = G == 1 ? mbar_wait(&acc_free[acc], (uint32_t)((done >> 1) & 1) ^ 1, wait_code + kUmmaWaitAccFree)
-                        : mbar_wait_cluster(&acc_free[acc], (uint32_t)((done >> 1) & 1) ^ 1, wait_code + kUmmaWaitAccFree);
+            ok = mbar_wait(&acc_free[acc], (uint32_t)((done >> 1) & 1) ^ 1, wait_code + kUmmaWaitAccFree);
             if (!ok) break;
             d = tmem + acc * C::BN;
           }
-          ok = G == 1 ? mbar_wait(&full[slot], round & 1, wait_code + kUmmaWaitFull)
-                      : mbar_wait_cluster(&full[slot], round & 1, wait_code + kUmmaWaitFull);
+          ok = mbar_wait(&full[slot], round & 1, wait_code + kUmmaWaitFull);
           if (!ok) break;
           tc_fence_after();
           const uint32_t a = smem_u32(smem + (size_t)slot * C::kStageBytes), b = a + C::PLANES * C::kABytes;
@@ -342,8 +340,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     uint32_t done = 0, tiles_done = 0;
     auto acquire = [&]() {
       const int acc = (int)(done & 1);
-      const bool got = G == 1 ? mbar_wait(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc)
-                              : mbar_wait_cluster(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc);
+      const bool got = mbar_wait(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc);
       tc_fence_after();
       return (bool)__all_sync(0xffffffffu, got);
     };
@@ -561,6 +558,40 @@ inline int encode_operand(CUtensorMap* map, const void* base, bool i8, long long
   return r == CUDA_SUCCESS ? BLB200_OK : BLB200_E_INTERNAL;
 }
 
+// How many clusters (or CTAs) of this kernel the current device holds at once: clusters do not straddle the device's groups of
+// SMs, so it is less than the number of SMs over the cluster's size.  Asked once per device and thread.
+template <class C, class Epilogue>
+int umma_capacity() {
+  constexpr int kCluster = C::GROUP * C::SPLIT;
+  if (kCluster == 1) return device_info().sm_count;
+  static thread_local int known[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) dev = 0;
+  if (known[dev] == 0) {
+    auto kern = umma_gemm_kernel<C, Epilogue>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kCluster);
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = UmmaMemory<C, Epilogue>::kBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)UmmaMemory<C, Epilogue>::kBytes) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = std::max(1, device_info().sm_count / kCluster - 4);
+    }
+    known[dev] = n;
+  }
+  return known[dev];
+}
+
 template <class C, class Epilogue>
 int launch_umma(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_old, const CUtensorMap& map_out, UmmaShape s, const typename Epilogue::Params& ep, int wait_code,
                 cudaStream_t stream, const PlainOperands& po = PlainOperands{}) {
@@ -580,7 +611,7 @@ int launch_umma(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtens
     configured_for = cur;
   }
   // a split tile has a cluster of its own, otherwise the CTAs or pairs that the device holds walk over the tiles
-  const long long units = C::SPLIT > 1 ? s.tiles : device_info().sm_count / C::GROUP;
+  const long long units = C::SPLIT > 1 ? s.tiles : umma_capacity<C, Epilogue>();
   if (units * kCluster > 0x7fffffffll) return BLB200_E_TOO_LARGE;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((s.tiles < units ? s.tiles : units) * kCluster));

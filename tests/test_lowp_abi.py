@@ -86,6 +86,9 @@ def test_newton_schulz_workspace_is_checked_before_any_launch(lib):
     assert lib.blb200_newton_schulz(d, 0x10000, need - 1, None) == _lib.E_SHAPE
     assert lib.blb200_newton_schulz(d, 0x10010, need, None) == _lib.E_SHAPE
     assert lib.blb200_newton_schulz_workspace_bytes(ns_desc(rows=0)) == 0
+    big = dict(rows=1024, cols=1024, ldx=1024, ldy=1024, batch=3, stride_x=1 << 20, stride_y=1 << 20)
+    assert lib.blb200_newton_schulz_workspace_bytes(ns_desc(steps=1, **big)) == \
+        lib.blb200_newton_schulz_workspace_bytes(ns_desc(steps=64, **big))   # one scratch serves every number of steps
     d.coefficients = None
     assert lib.blb200_newton_schulz(d, 0x10000, need, None) == _lib.E_NULL
 

@@ -62,7 +62,7 @@ def quantize_reference(x):
 
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("batch,cols,k", [(1, 1, 1), (1, 1, 16), (2, 3, 7), (1, 5, 33), (3, 17, 130), (1, 2, 4096), (2, 9, 1001),
-                                          (1, 1, 20000), (1, 700, 64), (1, 3, 70001)])
+                                          (1, 1, 20000), (1, 700, 64), (1, 3, 70001), (70000, 1, 3), (2, 33, 2048)])
 def test_quantize(bl, kind, batch, cols, k):
     x = (torch.randn(batch, cols, k, generator=gen(k + cols)) * torch.exp(3 * torch.randn(batch, cols, 1, generator=gen(k)))).to(TYPES[kind])
     x[0, 0, : k // 3] = x[0, 0].abs().max() / 2   # a tie: 63.5 steps
@@ -76,6 +76,22 @@ def test_quantize(bl, kind, batch, cols, k):
         assert np.array_equal(q.cpu().numpy(), want_q)
         q.fill_(7)
         assert bool((qb == 7).all()), "padding was written"
+
+
+@pytest.mark.parametrize("kind,bits", [("bf16", 8), ("f16", 11)])
+def test_quantize_every_halfway_point_of_the_half_types(bl, kind, bits):
+    """Every mantissa as the column's largest value, every mantissa below it in nine binades as an element."""
+    mantissas = np.arange(2 ** (bits - 1), 2 ** bits, dtype=np.float32) / 2 ** bits
+    values = (mantissas[:, None] * np.exp2(-np.arange(9, dtype=np.float32))).ravel()
+    for first in range(0, len(mantissas), 128):
+        tops = mantissas[first:first + 128, None]
+        x = np.where(values <= tops, values, 0)
+        x[:, ::2] *= -1
+        x[:, 0] = tops[:, 0]
+        d = torch.from_numpy(x.astype(np.float32))[None].to(TYPES[kind])
+        q, s = bl.quantize_i8(d.cuda())
+        want_q, want_s = quantize_reference(d.float().numpy())
+        assert np.array_equal(s.cpu().numpy(), want_s) and np.array_equal(q.cpu().numpy(), want_q)
 
 
 @pytest.mark.parametrize("kind", TYPES)
