@@ -185,12 +185,12 @@ struct I8Params {
 // tested for each element it was 36, and the epilogue, not the MMAs, set the time of an 8192^3 product).
 struct I8Epilogue {
   using Params = I8Params;
-  static constexpr bool kStaged = false;
+  static constexpr bool kStaged = false, kRows = false;
   static constexpr int kWarpBytesPerColumn = 4;
-  template <int W, int COLS>
+  template <int W, int COLS, int ROWS, int PLANE_BYTES>
   struct Tile;
 };
-template <int W, int COLS>
+template <int W, int COLS, int ROWS, int PLANE_BYTES>
 struct I8Epilogue::Tile {
   const I8Params& p;
   float* scales;
@@ -198,7 +198,7 @@ struct I8Epilogue::Tile {
   int n0;
   float sa;
   bool live;
-  __device__ __forceinline__ Tile(const Params& p_, const UmmaShape&, const UmmaTile& tile, bool, int m_, int n, unsigned char* scratch, int)
+  __device__ __forceinline__ Tile(const Params& p_, const UmmaShape&, const UmmaTile& tile, bool, int m_, int n, unsigned char* scratch, int, int)
       : p(p_), scales(reinterpret_cast<float*>(scratch)), item(tile.item), m(m_), n0(n), live(m_ < p_.g.m) {
     sa = p.g.scale_a && live ? p.g.scale_a[item * p.g.ssa + m] : 1.f;
     sa *= p.g.alpha;

@@ -116,94 +116,130 @@ __global__ void __launch_bounds__(256) ingest_kernel(Matrices g, const double* p
   }
 }
 
-// out = alpha * product + beta * old, left as half planes in the staging buffer (and stored across the diagonal as well when
-// the result is symmetric) or, by the last step, written in the caller's type and layout.
-template <typename T, int PLANES, bool LAST>
-struct NsEpilogue {
-  struct Params {
-    const float2* factors;
-    int has_old;  // 0: beta is not used
-    void* out;
-    long long out_ld, out_plane, out_item;
-  };
-  static constexpr bool kStaged = true, kStagedOut = !LAST;
+// The epilogue's parameters: out = alpha * product + beta * old.
+struct NsParams {
+  const float2* factors;
+  int has_old;  // 0: beta is not used
+  void* out;
+  long long out_ld, out_plane, out_item;
+};
+
+// Into half planes, row by row through the staging buffer: a thread's columns lie side by side in memory.  A symmetric result's
+// tiles below the diagonal are also stored across it, where a warp's rows lie side by side.
+template <int PLANES>
+struct NsInner {
+  using Params = NsParams;
+  static constexpr bool kStaged = true, kStagedOut = true, kRows = true;
   static constexpr int kWarpBytesPerColumn = 0;
-  // One thread's row of a tile, from column n0 on; `staged` is its element of column n0 in the staging buffer.
-  template <int W, int COLS>
+  template <int W, int COLS, int ROWS, int PLANE_BYTES>
   struct Tile {
+    static_assert(W == 16, "");
     const Params& p;
     const UmmaShape& s;
-    T* out;
-    T* mirror;
-    __half* staged;
-    int plane;
+    unsigned char* staged;  // this thread's row of the first box
+    __half* mirror;
     float alpha, beta;
-    int n0;
-    bool live;
-    __device__ __forceinline__ Tile(const Params& p_, const UmmaShape& s_, const UmmaTile& tile, bool twice, int m, int n, unsigned char* staged_,
-                                    int plane_bytes)
-        : p(p_), s(s_), staged(reinterpret_cast<__half*>(staged_)), plane(plane_bytes / 2), n0(n), live(m < s_.m) {
+    int n0, col0, swizzle;
+    __device__ __forceinline__ Tile(const Params& p_, const UmmaShape& s_, const UmmaTile& tile, bool twice, int m, int n, unsigned char* staging,
+                                    int row, int col)
+        : p(p_), s(s_), staged(staging + row * 128), n0(n), col0(col), swizzle(row & 7) {
       const float2 f = p.factors[tile.item];
       alpha = f.x;
       beta = p.has_old ? f.y : 0.f;
-      T* base = (T*)p.out + (long long)tile.item * p.out_item;
-      out = base + m;
-      mirror = twice && live ? base + (long long)m * p.out_ld : nullptr;
+      mirror = twice && m < s.m ? (__half*)p.out + (long long)tile.item * p.out_item + m : nullptr;
     }
-    // Columns n0 + c ... n0 + c + W - 1.
-    __device__ __forceinline__ void group(const uint32_t (&v)[W], int c) {
-      const int n = n0 + c;
-      __half* at = staged + c * 128;
-      float r[W];
+    // Columns n0 + c ... n0 + c + 15.
+    __device__ __forceinline__ void group(const uint32_t (&v)[16], int c) {
+      const int n = n0 + c, box = (col0 + c) >> 6, j = ((col0 + c) & 63) >> 3;
+      uint32_t hi[8], lo[8];  // pairs of halves
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        r[i] = alpha * __uint_as_float(v[i]);
+      for (int h = 0; h < 2; ++h) {
+        uint4* at = reinterpret_cast<uint4*>(staged + box * (ROWS * 128) + (((j + h) ^ swizzle) << 4));
+        uint4* at_lo = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(at) + PLANE_BYTES);
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = alpha * __uint_as_float(v[8 * h + i]);
         if (p.has_old) {
-          float was = __half2float(at[i * 128]);
-          if constexpr (PLANES == 2) was += __half2float(at[plane + i * 128]);
-          r[i] = fmaf(beta, was, r[i]);
-        }
-      }
-      if constexpr (LAST) {
-        if (!live) return;
-        T* to = out + (long long)n * p.out_ld;
+          const uint4 was = *at;
+          const uint32_t w[4] = {was.x, was.y, was.z, was.w};
+          uint32_t l[4] = {0, 0, 0, 0};
+          if constexpr (PLANES == 2) {
+            const uint4 low = *at_lo;
+            l[0] = low.x; l[1] = low.y; l[2] = low.z; l[3] = low.w;
+          }
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          if (n + i < s.n) *to = from_f32<T>(r[i]);
+          for (int i = 0; i < 4; ++i) {
+            float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            if constexpr (PLANES == 2) {
+              const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&l[i]));
+              f.x += g.x;
+              f.y += g.y;
+            }
+            r[2 * i] = fmaf(beta, f.x, r[2 * i]);
+            r[2 * i + 1] = fmaf(beta, f.y, r[2 * i + 1]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2 pair = __floats2half2_rn(r[2 * i], r[2 * i + 1]);
+          hi[4 * h + i] = *reinterpret_cast<const uint32_t*>(&pair);
+          if constexpr (PLANES == 2) {
+            const float2 f = __half22float2(pair);
+            const __half2 rest = __floats2half2_rn(r[2 * i] - f.x, r[2 * i + 1] - f.y);
+            lo[4 * h + i] = *reinterpret_cast<const uint32_t*>(&rest);
+          }
+        }
+        *at = make_uint4(hi[4 * h], hi[4 * h + 1], hi[4 * h + 2], hi[4 * h + 3]);
+        if constexpr (PLANES == 2) *at_lo = make_uint4(lo[4 * h], lo[4 * h + 1], lo[4 * h + 2], lo[4 * h + 3]);
+      }
+      if (mirror) {
+        __half* to = mirror + (long long)n * p.out_ld;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (n + i < s.n) {
+            to[0] = half_of(hi[i / 2], i & 1);
+            if constexpr (PLANES == 2) to[p.out_plane] = half_of(lo[i / 2], i & 1);
+          }
           to += p.out_ld;
         }
-      } else {
-        uint32_t hi[W / 2], lo[W / 2];  // pairs of halves
+      }
+    }
+  };
+};
+
+// The last step's, into the caller's type and layout: the rows are the fast index, so that a warp stores 32 consecutive elements
+// of a column whatever its alignment; the old values come column by column.
+template <typename T, int PLANES>
+struct NsLast {
+  using Params = NsParams;
+  static constexpr bool kStaged = true, kStagedOut = false, kRows = false;
+  static constexpr int kWarpBytesPerColumn = 0;
+  template <int W, int COLS, int ROWS, int PLANE_BYTES>
+  struct Tile {
+    const UmmaShape& s;
+    const __half* staged;
+    T* out;
+    long long ld;
+    float alpha, beta;
+    int n0;
+    bool live;
+    __device__ __forceinline__ Tile(const Params& p, const UmmaShape& s_, const UmmaTile& tile, bool, int m, int n, unsigned char* staging, int row,
+                                    int col)
+        : s(s_), staged(reinterpret_cast<const __half*>(staging) + col * 128 + row), ld(p.out_ld), n0(n), live(m < s_.m) {
+      const float2 f = p.factors[tile.item];
+      alpha = f.x;
+      beta = f.y;
+      out = (T*)p.out + (long long)tile.item * p.out_item + m;
+    }
+    __device__ __forceinline__ void group(const uint32_t (&v)[W], int c) {
+      if (!live) return;
+      T* to = out + (long long)(n0 + c) * ld;
 #pragma unroll
-        for (int i = 0; i < W; i += 2) {
-          const __half h0 = __float2half_rn(r[i]), h1 = __float2half_rn(r[i + 1]);
-          at[i * 128] = h0;
-          at[(i + 1) * 128] = h1;
-          hi[i / 2] = pack_halves(h0, h1);
-          if constexpr (PLANES == 2) {
-            const __half l0 = __float2half_rn(r[i] - __half2float(h0)), l1 = __float2half_rn(r[i + 1] - __half2float(h1));
-            at[plane + i * 128] = l0;
-            at[plane + (i + 1) * 128] = l1;
-            lo[i / 2] = pack_halves(l0, l1);
-          }
-        }
-        if (mirror) {
-#pragma unroll
-          for (int h = 0; h < W / 2; h += 4) {
-            if (n + 2 * h + 8 <= s.n) {
-              *reinterpret_cast<uint4*>(mirror + n + 2 * h) = make_uint4(hi[h], hi[h + 1], hi[h + 2], hi[h + 3]);
-              if constexpr (PLANES == 2)
-                *reinterpret_cast<uint4*>(mirror + p.out_plane + n + 2 * h) = make_uint4(lo[h], lo[h + 1], lo[h + 2], lo[h + 3]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (n + 2 * h + i < s.n) {
-                  mirror[n + 2 * h + i] = half_of(hi[h + i / 2], i & 1);
-                  if constexpr (PLANES == 2) mirror[p.out_plane + n + 2 * h + i] = half_of(lo[h + i / 2], i & 1);
-                }
-            }
-          }
-        }
+      for (int i = 0; i < W; ++i) {
+        float was = __half2float(staged[(c + i) * 128]);
+        if constexpr (PLANES == 2) was += __half2float(staged[PLANE_BYTES / 2 + (c + i) * 128]);
+        if (n0 + c + i < s.n) *to = from_f32<T>(fmaf(beta, was, alpha * __uint_as_float(v[i])));
+        to += ld;
       }
     }
   };
@@ -222,7 +258,7 @@ struct Maps {
     int box, staged;
     CUtensorMap map;
   };
-  Entry e[16];
+  Entry e[32];
   int used = 0;
   int get(const CUtensorMap** out, const HalfMatrix& a, int z, int box, int staged = 0) {
     for (int i = 0; i < used; ++i)
@@ -230,7 +266,7 @@ struct Maps {
         *out = &e[i].map;
         return BLB200_OK;
       }
-    if (used == 16) return BLB200_E_INTERNAL;  // four matrices in four boxes each at most
+    if (used == 32) return BLB200_E_INTERNAL;  // four matrices in six boxes each at most
     const int rc = encode_operand(&e[used].map, a.p, false, a.inner, a.outer, z, a.ld * 2, a.plane * 2, box, staged != 0);
     if (rc != BLB200_OK) return rc;
     e[used].p = a.p;
@@ -261,8 +297,9 @@ int launch_product(Maps& maps, const Operands& o, const typename Epilogue::Param
   int rc = maps.get(&map_a, o.a, z, A_MN ? 64 : 128);
   if (rc == BLB200_OK) rc = maps.get(&map_b, o.b, z, B_MN ? 64 : C::kBRows);
   map_old = map_out = map_a;
-  if (rc == BLB200_OK && ep.has_old) rc = maps.get(&map_old, o.old, z, kStagedColumns, 1);
-  if (rc == BLB200_OK && Epilogue::kStagedOut) rc = maps.get(&map_out, o.out, z, kStagedColumns, 1);
+  const int box = Epilogue::kRows ? 128 / SPLIT : kStagedColumns;
+  if (rc == BLB200_OK && ep.has_old) rc = maps.get(&map_old, o.old, z, box, !Epilogue::kRows);
+  if (rc == BLB200_OK && Epilogue::kStagedOut) rc = maps.get(&map_out, o.out, z, box, !Epilogue::kRows);
   if (rc == BLB200_OK) rc = launch_umma<C, Epilogue>(*map_a, *map_b, *map_old, *map_out, s, ep, kUmmaNsWait, stream);
   if (rc == BLB200_OK) note_launch("newton_schulz");
   return rc;
@@ -391,8 +428,8 @@ int run(const blb200_newton_schulz_desc* d, const Layout& l, char* ws, cudaStrea
   };
   int rc = wide ? passes(norm_parts_kernel<T, V>, ingest_kernel<T, V, PLANES>) : passes(norm_parts_kernel<T, 1>, ingest_kernel<T, 1, PLANES>);
   Maps maps;
-  using Inner = NsEpilogue<__half, PLANES, false>;
-  using Last = NsEpilogue<T, PLANES, true>;
+  using Inner = NsInner<PLANES>;
+  using Last = NsLast<T, PLANES>;
   for (int i = 0; i < d->steps && rc == BLB200_OK; ++i) {
     const float2* f = factors + (long long)i * 3 * batch;
     const typename Inner::Params gram{f, 0, s.p, l.ld_s, l.plane_s, PLANES * l.plane_s};
@@ -402,15 +439,17 @@ int run(const blb200_newton_schulz_desc* d, const Layout& l, char* ws, cudaStrea
     const typename Inner::Params square{f + batch, 1, b.p, l.ld_s, l.plane_s, PLANES * l.plane_s};
     rc = product<false, false, PLANES, Inner>(maps, Operands{s, s, s, b, p, p, p, batch, true}, square, stream);
     if (rc != BLB200_OK) break;
-    const Operands update_o{r <= c ? b : x, r <= c ? x : b, x, x2, r, c, p, batch, false};
     if (i + 1 < d->steps) {
+      // the columns of X as the tile's rows, so that the epilogue goes along memory
       const typename Inner::Params update{f + 2 * batch, 1, x2.p, l.ld_x, l.plane_x, PLANES * l.plane_x};
+      const Operands update_o{r <= c ? x : b, r <= c ? b : x, x, x2, c, r, p, batch, false};
       rc = r <= c ? product<false, false, PLANES, Inner>(maps, update_o, update, stream)
-                  : product<true, false, PLANES, Inner>(maps, update_o, update, stream);
+                  : product<false, true, PLANES, Inner>(maps, update_o, update, stream);
       std::swap(x, x2);
     } else {
       const typename Last::Params last{f + 2 * batch, 1, d->y, d->ldy, 0, d->stride_y};
-      rc = r <= c ? product<false, false, PLANES, Last>(maps, update_o, last, stream) : product<true, false, PLANES, Last>(maps, update_o, last, stream);
+      const Operands last_o{r <= c ? b : x, r <= c ? x : b, x, x2, r, c, p, batch, false};
+      rc = r <= c ? product<false, false, PLANES, Last>(maps, last_o, last, stream) : product<true, false, PLANES, Last>(maps, last_o, last, stream);
     }
   }
   return rc;

@@ -24,8 +24,9 @@
 //
 // Epilogue: a thread owns one row of the tile (32 consecutive rows per warp) and takes its columns in groups of sixteen, in a
 // rolled loop: unrolled over the tile the code is 10 KB and more, which a kernel of a few microseconds spends its time
-// fetching (128 x 128 tiles: 2.3 us of 5.6).  A staged epilogue reads the old values of the result's tile from, and leaves the new
-// ones in, a buffer of half columns (128 rows each) that tensor-map copies fill while the products run and write out.
+// fetching (128 x 128 tiles: 2.3 us of 5.6).  A staged epilogue reads the old values of the result's tile from, and may leave the new
+// ones in, a buffer that tensor-map copies fill while the products run and write out: row-wise, where the columns are the fast
+// index in memory (sixteen values are two 16-byte accesses), or column by column.
 //
 // A wait that runs out records its code, and the role leaves its loop; the other roles' waits then run out as well, the
 // copies still in flight are waited for, tensor memory is freed and the kernel returns.
@@ -47,7 +48,7 @@ struct UmmaShape {
 };
 
 enum UmmaWait { kUmmaWaitEmpty = 1, kUmmaWaitFull = 2, kUmmaWaitAccFree = 3, kUmmaWaitAcc = 4, kUmmaWaitDrain = 5, kUmmaWaitStaging = 6, kUmmaWaitOld = 7 };
-constexpr int kStagedColumns = 32;  // columns per box of the staging buffer
+constexpr int kStagedColumns = 32;  // columns per box of a column-wise staging buffer
 
 template <bool I8_, bool A_MN_, bool B_MN_, int GROUP_, int BN_, int PLANES_, int SPLIT_ = 1, bool PLAIN_ = false>
 struct UmmaConfig {
@@ -216,8 +217,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   if constexpr (kCluster > 1) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // Everything above may overlap the end of the kernel before this one; its results are read from here on.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // The kernel before this one may still run: its results are read after a wait, which each role puts where it needs them.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 0) {
@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             else tma_load_3d(dst, map, x, y, z, &full[slot]);
           };
           const int k0 = (kb_begin + kb) * C::kKStage;
+          if (t == first && kb == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 #pragma unroll
           for (int pl = 0; pl < C::PLANES; ++pl) {
             unsigned char* a = stage + pl * C::kABytes;
@@ -332,10 +333,18 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
     }
   } else {
-    // Two warps per quarter of the 128 rows: each takes half of the columns.
-    constexpr int kCols = C::BN / 2, kOwn = C::BN / C::SPLIT, kMine = kOwn / 2, W = kMine < 16 ? kMine : 16;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // Two warps per quarter of the 128 rows of the accumulator: each takes half of the columns.  Of a split tile a CTA stores
+    // some of the rows (row-wise epilogues) or of the columns, cut the same way over the warps.
+    constexpr bool kRows = Epilogue::kRows;
+    constexpr int kCols = C::BN / 2, kOwnRows = kRows ? 128 / C::SPLIT : 128, kOwnCols = kRows ? C::BN : C::BN / C::SPLIT;
+    constexpr int kRowParts = kOwnRows / 32, kMine = kOwnCols * kRowParts / 8, W = kMine < 16 ? kMine : 16;
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const int row = quarter * 32 + lane;
+    const int own_row = C::SPLIT > 1 ? ((warp - 2) % kRowParts) * 32 + lane : row;
+    const int own_col = (C::SPLIT > 1 ? (warp - 2) / kRowParts : half) * kMine;
+    const int first_row = (int)rank * 128 + (C::SPLIT > 1 && kRows ? (int)cta * kOwnRows : 0);  // of what this CTA stores
+    const int first_col = C::SPLIT > 1 && !kRows ? (int)cta * kOwnCols : 0;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + half * kCols;
     uint32_t done = 0, tiles_done = 0;
     auto acquire = [&]() {
@@ -353,14 +362,19 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
       ++done;
     };
-    // The staging buffer's owner sends for a tile's old values as soon as the tile before has left it.
-    auto request_old = [&](int t) {
-      const UmmaTile tile = umma_tile<C::kRatio>(s, t);
-      mbar_arrive_expect_tx(old_full, C::PLANES * kOwn * 256);
+    // The staging buffer: boxes of 64 columns, rows of 128 bytes in the 128-byte swizzle (row-wise), or of kStagedColumns columns of
+    // 128 rows.  Its owner sends for a tile's old values as soon as the tile before has left it.
+    constexpr int kBoxCols = kRows ? 64 : kStagedColumns, kBoxBytes = kOwnRows * kBoxCols * 2, kPlaneBytes = kOwnRows * kOwnCols * 2;
+    auto boxes = [&](const UmmaTile& tile, auto each) {
       for (int pl = 0; pl < C::PLANES; ++pl)
-        for (int c = 0; c < kOwn; c += kStagedColumns)
-          tma_load_3d(staging + (pl * kOwn + c) * 256, &map_old, tile.tm * C::kBM + (int)rank * 128,
-                      tile.tn * C::BN + (C::SPLIT > 1 ? (int)cta * kOwn : 0) + c, tile.item * C::PLANES + pl, old_full);
+        for (int c = 0; c < kOwnCols; c += kBoxCols) {
+          const int n = tile.tn * C::BN + first_col + c, m = tile.tm * C::kBM + first_row;
+          each(staging + pl * kPlaneBytes + c / kBoxCols * kBoxBytes, kRows ? n : m, kRows ? m : n, tile.item * C::PLANES + pl, n < s.n && m < s.m);
+        }
+    };
+    auto request_old = [&](int t) {
+      mbar_arrive_expect_tx(old_full, C::PLANES * kPlaneBytes);
+      boxes(umma_tile<C::kRatio>(s, t), [&](unsigned char* at, int x, int y, int z, bool) { tma_load_3d(at, &map_old, x, y, z, old_full); });
     };
     if constexpr (Epilogue::kStaged) {
       if (threadIdx.x == 64 && ep.has_old && first < s.tiles) request_old(first);
@@ -416,11 +430,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         }
         fetched = ok;
       }
-      const int m = tile.tm * C::kBM + (int)rank * 128 + row;
-      const int mine = tile.tn * C::BN + (C::SPLIT > 1 ? (int)cta * kOwn : 0) + half * kMine;  // first of this thread's columns
+      const int m = tile.tm * C::kBM + first_row + own_row, mine = tile.tn * C::BN + first_col + own_col;
       const bool twice = s.symmetric && tile.tn < C::kRatio * tile.tm;
-      unsigned char* scratch = Epilogue::kStaged ? staging + half * kMine * 256 + row * 2 : staging + (warp - 2) * (M::kStaging / 8);
-      typename Epilogue::template Tile<W, kMine> epi(ep, s, tile, twice, m, mine, scratch, kOwn * 256);
+      unsigned char* scratch = Epilogue::kStaged ? staging : staging + (warp - 2) * (M::kStaging / 8);
+      typename Epilogue::template Tile<W, kMine, kOwnRows, kPlaneBytes> epi(ep, s, tile, twice, m, mine, scratch, own_row, own_col);
       if constexpr (C::kChunk == 0) {
         ok = k_blocks == 0 || acquire();
       } else if (k_blocks > 0) {
@@ -462,8 +475,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         }
         release();
       } else {
-        // The cluster has this one tile.  Once every CTA is past its products the stages are free: column c goes to the CTA
-        // c / kOwn, into its slab for this CTA.
+        // The cluster has this one tile.  Once every CTA is past its products the stages are free: each element goes to the CTA that
+        // stores it, into its slab for this CTA.
         cluster_sync();
 #pragma unroll 1
         for (int c = 0; c < kCols; c += 16) {
@@ -475,7 +488,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int col = half * kCols + c + i;
-            const uint32_t to = cluster_addr(smem_u32(smem), col / kOwn) + ((cta * kOwn + col % kOwn) * 128 + row) * 4;
+            const uint32_t to = cluster_addr(smem_u32(smem), kRows ? row / kOwnRows : col / kOwnCols) +
+                                ((cta * kOwnCols + col % kOwnCols) * kOwnRows + row % kOwnRows) * 4;
             asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(v[i]) : "memory");
           }
         }
@@ -488,11 +502,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           uint32_t v[W];
 #pragma unroll
           for (int i = 0; i < W; ++i) {
-            const int col = half * kMine + c + i;
-            v[i] = sums[col * 128 + row];
+            const int col = own_col + c + i;
+            v[i] = sums[col * kOwnRows + own_row];
 #pragma unroll
             for (int from = 1; from < C::SPLIT; ++from) {
-              const uint32_t w = sums[(from * kOwn + col) * 128 + row];
+              const uint32_t w = sums[(from * kOwnCols + col) * kOwnRows + own_row];
               v[i] = C::I8 ? v[i] + w : __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(w));
             }
           }
@@ -504,11 +518,9 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         named_all(true, 256);
         if (threadIdx.x == 64) {
           if constexpr (Epilogue::kStagedOut) {
-            const int first_col = tile.tn * C::BN + (C::SPLIT > 1 ? (int)cta * kOwn : 0);
-            for (int pl = 0; pl < C::PLANES; ++pl)
-              for (int c = 0; c < kOwn; c += kStagedColumns)
-                if (first_col + c < s.n && tile.tm * C::kBM + (int)rank * 128 < s.m)
-                  tma_store_3d(&map_out, staging + (pl * kOwn + c) * 256, tile.tm * C::kBM + (int)rank * 128, first_col + c, tile.item * C::PLANES + pl);
+            boxes(tile, [&](unsigned char* at, int x, int y, int z, bool exists) {
+              if (exists) tma_store_3d(&map_out, at, x, y, z);
+            });
             bulk_commit();
             bulk_wait_read<0>();
           }
