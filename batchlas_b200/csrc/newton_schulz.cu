@@ -325,7 +325,7 @@ int product(Maps& maps, const Operands& o, const typename Epilogue::Params& ep, 
   const double single = rounds(tiles(128, 128), sms) * (blocks * block + 12);
   const long long most[2] = {umma_capacity<UmmaConfig<false, A_MN, B_MN, 1, 128, PLANES, 2>, Epilogue>(),
                              umma_capacity<UmmaConfig<false, A_MN, B_MN, 1, 128, PLANES, 4>, Epilogue>()};
-  auto split = [&](int s) { return tiles(128, 128) > most[s / 4] ? 1e300 : (double)((blocks + s - 1) / s) * block + 18; };
+  auto split = [&](int s) { return tiles(128, 128) > most[s / 4] ? 1e300 : (double)((blocks + s - 1) / s) * block + 15; };
   const double best = std::min(std::min(pair, single), std::min(split(2), split(4)));
   if (best == pair) return launch_product<A_MN, B_MN, 2, kPairN, PLANES, 1, Epilogue>(maps, o, ep, stream);
   if (best == single) return launch_product<A_MN, B_MN, 1, 128, PLANES, 1, Epilogue>(maps, o, ep, stream);

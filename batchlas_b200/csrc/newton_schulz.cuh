@@ -37,12 +37,12 @@ __host__ __device__ inline double polynomial_bound(const double* q, double top) 
 }
 
 __device__ __forceinline__ double block_sum(double v) {
-  __shared__ double part[8];
+  __shared__ double part[32];
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0;
-  for (int i = 0; i < 8; ++i) v += part[i];
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) v += part[i];
   __syncthreads();
   return v;
 }

@@ -1,7 +1,7 @@
 // The Newton-Schulz iteration on small matrices: one CTA per matrix, everything but G and the result in its shared memory.
 //
 // Per step  S = X X^T,  B = b S + c S^2,  X <- a X + B X  are three tcgen05 products of one 128-row tile, issued by one thread,
-// each followed by an epilogue of all eight warps that scales the accumulator in tensor memory and writes the next operand.
+// each followed by an epilogue of all sixteen warps that scales the accumulator in tensor memory and writes the next operand.
 // X (p x q, p the shorter side, padded with zeros to 128 x 64 QB) lies as blocks of 64 columns of 128 rows of 128 bytes in the
 // 128-byte swizzle: read as rows of q that is the K-major operand of X X^T, and read as rows of 64 q per p it is the
 // MN-major operand of B X, so it is never transposed.  S and B share one place: both S and X are only overwritten, element by
@@ -17,7 +17,7 @@ namespace blb200 {
 namespace {
 
 enum SmallWait { kSmallWait = 651 };
-constexpr int kThreads = 256;
+constexpr int kThreads = 512, kParts = kThreads / 128;  // warps per quarter of the rows
 
 template <int PLANES, int QB>
 struct SmallMemory {
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kThreads) newton_schulz_small_kernel(Matrices 
     if (threadIdx.x == 0) {
       const uint32_t idesc = umma_idesc(false, false, b_mn, 128, n);
       const uint32_t lead = b_mn ? 16384 : 16;
-#pragma unroll 1
+#pragma unroll 4
       for (int k = 0; k < k_steps; ++k) {
         const uint32_t step = (k >> 2) * 16384 + (k & 3) * 32, step_b = b_mn ? k * 2048 : step;
         const uint64_t da = umma_desc(smem_u32(a) + step, 16, 1024), db = umma_desc(smem_u32(b) + step_b, lead, 1024);
@@ -103,9 +103,9 @@ __global__ void __launch_bounds__(kThreads) newton_schulz_small_kernel(Matrices 
     tc_fence_after();
     return __syncthreads_and(done) != 0;
   };
-  // Each thread takes one row of the tile and half of its columns, sixteen at a time: out = alpha * product + beta * old, old
+  // Each thread takes one row of the tile and a quarter of its columns, sixteen at a time: out = alpha * product + beta * old, old
   // and out at the same place of `at`.
-  const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+  const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
   const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
   auto sixteen = [&](unsigned char* at, int plane, int c, float2 f, bool has_old, float (&r)[16]) {
     uint32_t v[16];
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads) newton_schulz_small_kernel(Matrices 
   };
   auto epilogue = [&](unsigned char* at, int plane, int columns, float2 f, bool has_old) {
 #pragma unroll 1
-    for (int c = half * (columns / 2); c < (half + 1) * (columns / 2); c += 16) {
+    for (int c = part * (columns / kParts); c < (part + 1) * (columns / kParts); c += 16) {
       float r[16];
       sixteen(at, plane, c, f, has_old, r);
 #pragma unroll
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads) newton_schulz_small_kernel(Matrices 
       const int p = wide ? y.rows : y.cols, q = wide ? y.cols : y.rows;
       const long long to_row = wide ? 1 : y.ld, to_col = wide ? y.ld : 1;
 #pragma unroll 1
-      for (int c = half * (QB * 32); c < (half + 1) * (QB * 32) && c < q; c += 16) {
+      for (int c = part * (QB * 64 / kParts); c < (part + 1) * (QB * 64 / kParts) && c < q; c += 16) {
         float r[16];
         sixteen(x, M::kX, c, f[2], true, r);
         if (row < p) {
