@@ -327,7 +327,7 @@ int validate_gemm_i8(const blb200_gemm_i8_desc* d) {
   if (!d) return BLB200_E_NULL;
   if (!valid_ftype(d->ftype_c)) return BLB200_E_DTYPE;
   if (d->m < 0 || d->n < 0 || d->k < 0 || d->batch < 0) return BLB200_E_SHAPE;
-  if (d->k > kMaxK) return BLB200_E_TOO_LARGE;
+  if (d->k > kMaxK || d->m > kMaxDim || d->n > kMaxDim) return BLB200_E_TOO_LARGE;
   if (!readable_layout(d->k, d->lda, d->stride_a) || !readable_layout(d->k, d->ldb, d->stride_b) ||
       !writable_layout(d->m, d->n, d->batch, d->ldc, d->stride_c) || d->stride_scale_a < 0 || d->stride_scale_b < 0)
     return BLB200_E_SHAPE;

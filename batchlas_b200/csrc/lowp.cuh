@@ -32,6 +32,9 @@ int with_ftype(int t, F&& f) {
   return f(__nv_bfloat16{});
 }
 
+// Largest dimension of these calls: coordinates and loop counters past it may reach the end of 32 bits.
+constexpr int kMaxDim = 1 << 30;
+
 // ld and stride of a column-major operand that is read: items may overlap or coincide.
 inline bool readable_layout(long long rows, long long ld, long long stride) {
   return ld >= (rows > 1 ? rows : 1) && stride >= 0;

@@ -339,7 +339,7 @@ int validate_ns(const blb200_newton_schulz_desc* d) {
   if (d->rows < 0 || d->cols < 0 || d->batch < 0) return BLB200_E_SHAPE;
   if (!readable_layout(d->rows, d->ldx, d->stride_x) || !writable_layout(d->rows, d->cols, d->batch, d->ldy, d->stride_y))
     return BLB200_E_SHAPE;
-  if (d->batch > 65535) return BLB200_E_TOO_LARGE;
+  if (d->batch > 65535 || d->rows > kMaxDim || d->cols > kMaxDim) return BLB200_E_TOO_LARGE;
   if (d->steps < 1 || d->steps > kMaxSteps || !(d->eps >= 0.0) || !isfinite(d->eps)) return BLB200_E_UNSUPPORTED;
   if (!d->coefficients) return BLB200_E_NULL;
   if (d->coefficient_sets != 1 && d->coefficient_sets != d->steps) return BLB200_E_UNSUPPORTED;

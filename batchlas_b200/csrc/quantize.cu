@@ -263,6 +263,7 @@ int validate_quantize(const blb200_quantize_desc* d) {
   if (!d) return BLB200_E_NULL;
   if (!valid_ftype(d->ftype)) return BLB200_E_DTYPE;
   if (d->k < 0 || d->cols < 0 || d->batch < 0) return BLB200_E_SHAPE;
+  if (d->k > kMaxDim || d->cols > kMaxDim) return BLB200_E_TOO_LARGE;
   if (!readable_layout(d->k, d->ldx, d->stride_x) || !writable_layout(d->k, d->cols, d->batch, d->ldq, d->stride_q) ||
       !writable_layout(1, d->cols, d->batch, 1, d->stride_scale))
     return BLB200_E_SHAPE;

@@ -7,8 +7,8 @@ import ctypes
 
 import torch
 
-from ._lib import NewtonSchulzDesc, check, load
-from .quantized import FTYPE_CODES, _matrix, _same_device
+from ._lib import NewtonSchulzDesc, load
+from .quantized import FTYPE_CODES, _launch, _matrix, _same_device
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
 
@@ -21,7 +21,7 @@ def _desc(X, Y, steps, coefficients, eps):
     if (batch, cols, rows) != (y_batch, y_cols, y_rows):
         raise RuntimeError("NEWTON_SCHULZ: incompatible matrix dimensions")
     sets = list(coefficients)
-    if len(sets) == 3 and all(isinstance(v, (int, float)) for v in sets):
+    if len(sets) == 3 and isinstance(sets[0], (int, float)):
         sets = [sets]
     if len(sets) not in (1, steps) or any(len(s) != 3 for s in sets):
         raise ValueError("newton_schulz: coefficients are one triple (a, b, c), or one for each step")
@@ -45,19 +45,18 @@ def newton_schulz(X, Y=None, steps=5, coefficients=QUINTIC, eps=1e-7, *, workspa
     :func:`newton_schulz_workspace_bytes` bytes) is given.  Asynchronous."""
     if Y is None:
         Y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
-    _same_device("batchlas_b200.newton_schulz", X.get_device(), Y)
+    index = X.get_device()
+    _same_device("batchlas_b200.newton_schulz", index, Y)
     d = _desc(X, Y, steps, coefficients, eps)
-    with torch.cuda.device(Y.device):
-        need = int(load().blb200_newton_schulz_workspace_bytes(d))
+    need = int(load().blb200_newton_schulz_workspace_bytes(d))
+    if workspace is None:
         if stream is None:
-            run_on = torch.cuda.current_stream()
-        else:
-            run_on = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
-        if workspace is None:
-            with torch.cuda.stream(run_on):  # the scratch belongs to the stream that uses it
-                workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=Y.device)
-        elif workspace.device != Y.device or workspace.dtype != torch.uint8 or workspace.numel() < need \
-                or not workspace.is_contiguous() or workspace.data_ptr() % 256:
-            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {Y.device}, 256-byte aligned")
-        check(load().blb200_newton_schulz(d, workspace.data_ptr(), workspace.numel(), run_on.cuda_stream))
+            workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=X.device)
+        else:  # the scratch belongs to the stream that uses it
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, X.device) if stream else torch.cuda.default_stream(X.device)):
+                workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=X.device)
+    elif workspace.get_device() != index or workspace.dtype is not torch.uint8 or workspace.numel() < need \
+            or not workspace.is_contiguous() or workspace.data_ptr() % 256:
+        raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {X.device}, 256-byte aligned")
+    _launch(index, stream, lambda desc, on: load().blb200_newton_schulz(desc, workspace.data_ptr(), workspace.numel(), on), d)
     return Y

@@ -22,6 +22,8 @@
 // (src/util/sycl-util-impl.cc:36-46) — so tests can index elements on the host after ctx.wait().
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -1029,6 +1031,96 @@ inline Matrix<T> matmul(Queue& ctx, const MatrixView<T, MatrixFormat::Dense>& A,
   return C;
 }
 }  // namespace linalg
+
+// ---- products in the types of language models' layers ---------------------------------------------
+// 8-bit integer products with scales per channel and token, their quantiser, and the Newton-Schulz orthogonalisation of
+// update matrices (no counterpart in BatchLAS; semantics in blb200.h).  Scales are VectorViews of float with inc 1.
+namespace detail {
+template <typename T>
+constexpr int ftype_code() {
+  if constexpr (std::is_same_v<T, float>) return BLB200_F32;
+  else if constexpr (std::is_same_v<T, __half>) return BLB200_F16;
+  else {
+    static_assert(std::is_same_v<T, __nv_bfloat16>, "float, __half or __nv_bfloat16");
+    return BLB200_BF16;
+  }
+}
+inline int64_t scale_stride(const char* name, const VectorView<float>& s, int size, int batch) {
+  if (s.size() != size || s.inc() != 1 || (s.batch_size() != batch && s.batch_size() != 1))
+    throw std::runtime_error(std::string(name) + ": incompatible scale dimensions");
+  return s.batch_size() == 1 ? 0 : s.stride();
+}
+}  // namespace detail
+
+struct GemmI8Options {
+  double alpha = 1.0;
+  double beta = 0.0;
+};
+struct NewtonSchulzOptions {
+  int steps = 5;
+  std::vector<double> coefficients = {3.4445, -4.7750, 2.0315};  // one triple, or one for each step
+  double eps = 1e-7;
+};
+
+// Q and scale <- every column of X quantised.
+template <typename T>
+inline Event quantize_i8(Queue& ctx, const MatrixView<T, MatrixFormat::Dense>& X, const MatrixView<int8_t, MatrixFormat::Dense>& Q,
+                         const VectorView<float>& scale) {
+  if (X.rows() != Q.rows() || X.cols() != Q.cols() || X.batch_size() != Q.batch_size())
+    throw std::runtime_error("QUANTIZE_I8: incompatible matrix dimensions");
+  blb200_quantize_desc d{};
+  d.x = X.data_ptr(); d.q = Q.data_ptr(); d.scale = scale.data_ptr();
+  d.k = X.rows(); d.cols = X.cols(); d.batch = X.batch_size();
+  d.ldx = X.ld(); d.stride_x = X.stride(); d.ldq = Q.ld(); d.stride_q = Q.stride();
+  d.stride_scale = detail::scale_stride("QUANTIZE_I8", scale, d.cols, d.batch);
+  d.ftype = detail::ftype_code<T>();
+  ctx.make_current();
+  detail::status_check(blb200_quantize_i8(&d, ctx.native_stream()));
+  return ctx.create_event_after_external_work();
+}
+
+// C <- alpha diag(scale_a) A^T B diag(scale_b) + beta C; a scale without data stands for ones.
+template <typename T>
+inline Event gemm_i8(Queue& ctx, const MatrixView<int8_t, MatrixFormat::Dense>& A, const MatrixView<int8_t, MatrixFormat::Dense>& B,
+                     const MatrixView<T, MatrixFormat::Dense>& C, const VectorView<float>& scale_a, const VectorView<float>& scale_b,
+                     const GemmI8Options& o = {}) {
+  blb200_gemm_i8_desc d{};
+  d.m = C.rows(); d.n = C.cols(); d.k = A.rows(); d.batch = C.batch_size();
+  if (A.cols() != d.m || B.cols() != d.n || B.rows() != d.k || (A.batch_size() != d.batch && A.batch_size() != 1) ||
+      (B.batch_size() != d.batch && B.batch_size() != 1))
+    throw std::runtime_error("GEMM_I8: incompatible matrix dimensions");
+  d.a = A.data_ptr(); d.b = B.data_ptr(); d.c = C.data_ptr();
+  d.lda = A.ld(); d.ldb = B.ld(); d.ldc = C.ld();
+  d.stride_a = A.batch_size() == 1 ? 0 : A.stride(); d.stride_b = B.batch_size() == 1 ? 0 : B.stride(); d.stride_c = C.stride();
+  d.scale_a = scale_a.data_ptr(); d.scale_b = scale_b.data_ptr();
+  if (d.scale_a) d.stride_scale_a = detail::scale_stride("GEMM_I8", scale_a, d.m, d.batch);
+  if (d.scale_b) d.stride_scale_b = detail::scale_stride("GEMM_I8", scale_b, d.n, d.batch);
+  d.alpha = o.alpha; d.beta = o.beta;
+  d.ftype_c = detail::ftype_code<T>();
+  ctx.make_current();
+  detail::status_check(blb200_gemm_i8(&d, ctx.native_stream()));
+  return ctx.create_event_after_external_work();
+}
+
+// Y <- the orthogonalised X (Y may be X); the scratch is leased from the queue's arena.
+template <typename T>
+inline Event newton_schulz(Queue& ctx, const MatrixView<T, MatrixFormat::Dense>& X, const MatrixView<T, MatrixFormat::Dense>& Y,
+                           const NewtonSchulzOptions& o = {}) {
+  if (X.rows() != Y.rows() || X.cols() != Y.cols() || X.batch_size() != Y.batch_size() || o.coefficients.size() % 3 != 0)
+    throw std::runtime_error("NEWTON_SCHULZ: incompatible matrix dimensions");
+  blb200_newton_schulz_desc d{};
+  d.x = X.data_ptr(); d.y = Y.data_ptr();
+  d.rows = X.rows(); d.cols = X.cols(); d.batch = X.batch_size();
+  d.ldx = X.ld(); d.ldy = Y.ld(); d.stride_x = X.stride(); d.stride_y = Y.stride();
+  d.ftype = detail::ftype_code<T>();
+  d.steps = o.steps; d.coefficient_sets = (int)(o.coefficients.size() / 3);
+  d.coefficients = o.coefficients.data();
+  d.eps = o.eps;
+  ctx.make_current();
+  WorkspaceLease ws = ctx.workspace(std::max<size_t>(blb200_newton_schulz_workspace_bytes(&d), 256));
+  detail::status_check(blb200_newton_schulz(&d, ws.data(), ws.size(), ctx.native_stream()));
+  return ctx.create_event_after_external_work();
+}
 
 }  // namespace batchlas
 

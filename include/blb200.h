@@ -337,7 +337,8 @@ typedef enum { BLB200_F32 = 0, BLB200_F16 = 1, BLB200_BF16 = 2 } blb200_ftype;
  * whose scale is 0 gets zeros (so an empty or all-zero column is exact); a column that holds a NaN or
  * an infinity gets that as its scale, and zeros, so a product made with it is NaN there.
  * scale: float, element j of item b at scale[b*stride_scale + j].  x, q and scale must not overlap.
- * Padding rows (>= k within ldq) are not written. */
+ * Padding rows (>= k within ldq) are not written.  (Dimensions of these three calls go up to 2^30, beyond that
+ * BLB200_E_TOO_LARGE.) */
 typedef struct blb200_quantize_desc {
   const void* x;
   int8_t* q;
@@ -353,8 +354,9 @@ int blb200_quantize_i8(const blb200_quantize_desc* desc, void* cuda_stream);
  * `ftype_c`.  The sums over k are exact 32-bit integers, hence k <= 131071, else BLB200_E_TOO_LARGE; the scales,
  * alpha and beta are applied in float, and C is rounded once.  A null scale pointer stands for ones.
  * stride_a, stride_b and the scales' strides may be 0 (one operand for the whole batch).
- * m == 0 or n == 0 is a no-op, k == 0 scales C by beta, beta == 0 never reads C.  Operands whose base, ld and stride
- * are multiples of 16 bytes take the tensor-map kernels, others the same sums at a lower rate. */
+ * m == 0 or n == 0 is a no-op, k == 0 scales C by beta, beta == 0 never reads C.  C must not overlap A, B or the scales.
+ * Operands whose base, ld and stride are multiples of 16 bytes are fetched by tensor-map copies, others by plain loads,
+ * for the same sums at a lower rate. */
 typedef struct blb200_gemm_i8_desc {
   const int8_t* a;
   const int8_t* b;
@@ -373,9 +375,10 @@ int blb200_gemm_i8(const blb200_gemm_i8_desc* desc, void* cuda_stream);
  *     X <- G / (||G||_F + eps);   steps times:  S = X X^T,  X <- (a I + b S + c S^2) X      (rows <= cols;
  * X^T X from the right otherwise), and writes the last X to y (y may be x itself, same ld and stride).
  * coefficients: (a, b, c) once (coefficient_sets 1) or one triple per step (coefficient_sets == steps).
+ * float and float16 keep every intermediate matrix as a pair of float16 matrices (float accuracy), bfloat16 as one.
  * From the coefficients follows a bound on X's largest singular value at each step; coefficients under
  * which it passes 64, or an entry of b S + c S^2 may pass 16384, are refused with BLB200_E_TOO_LARGE.
- * steps 1 .. 64, eps >= 0.  An item that holds a NaN or an infinity comes out as NaN.
+ * steps 1 .. 64, eps >= 0, batch <= 65535.  An item that holds a NaN or an infinity comes out as NaN.
  * workspace: device memory of at least blb200_newton_schulz_workspace_bytes, 256-byte aligned. */
 typedef struct blb200_newton_schulz_desc {
   const void* x;

@@ -49,7 +49,8 @@ def test_descriptor_layouts_match_the_header():
     (dict(batch=-1), _lib.E_SHAPE), (dict(ldx=7), _lib.E_SHAPE), (dict(ldq=7), _lib.E_SHAPE), (dict(stride_x=-1), _lib.E_SHAPE),
     (dict(stride_q=0), _lib.E_SHAPE), (dict(stride_q=31), _lib.E_SHAPE), (dict(stride_scale=3), _lib.E_SHAPE),
     (dict(x=0), _lib.E_NULL), (dict(q=0), _lib.E_NULL), (dict(scale=0), _lib.E_NULL),
-    (dict(cols=0, x=0, q=0, scale=0), 0), (dict(batch=0), 0)])
+    (dict(cols=0, x=0, q=0, scale=0), 0), (dict(batch=0), 0),
+    (dict(k=(1 << 30) + 1, ldx=1 << 31, ldq=1 << 31, stride_x=1 << 34, stride_q=1 << 34), _lib.E_TOO_LARGE)])
 def test_quantize_refusals(lib, kw, status):
     assert lib.blb200_quantize_i8(quantize_desc(**kw), None) == status
 
@@ -60,7 +61,8 @@ def test_quantize_refusals(lib, kw, status):
     (dict(ldc=3), _lib.E_SHAPE), (dict(batch=2), _lib.E_SHAPE), (dict(batch=2, stride_c=15), _lib.E_SHAPE),
     (dict(batch=2, stride_c=4, ldc=7), _lib.E_SHAPE), (dict(stride_scale_a=-1), _lib.E_SHAPE),
     (dict(a=0), _lib.E_NULL), (dict(b=0), _lib.E_NULL), (dict(c=0), _lib.E_NULL),
-    (dict(m=0, a=0, b=0, c=0), 0), (dict(n=0), 0), (dict(batch=0), 0)])
+    (dict(m=0, a=0, b=0, c=0), 0), (dict(n=0), 0), (dict(batch=0), 0),
+    (dict(m=(1 << 30) + 1, ldc=1 << 31), _lib.E_TOO_LARGE), (dict(n=(1 << 30) + 1), _lib.E_TOO_LARGE)])
 def test_gemm_i8_refusals(lib, kw, status):
     assert lib.blb200_gemm_i8(gemm_desc(**kw), None) == status
 
@@ -73,7 +75,8 @@ def test_gemm_i8_refusals(lib, kw, status):
     (dict(coefficients=(float("inf"), 0.0, 0.0)), _lib.E_UNSUPPORTED), (dict(coefficients=(65.0, 0.0, 0.0)), _lib.E_TOO_LARGE),
     (dict(coefficients=(3.0, 0.0, 0.0)), _lib.E_TOO_LARGE),          # 3^5 > 64
     (dict(coefficients=(1.0, 20000.0, -20000.0)), _lib.E_TOO_LARGE),
-    (dict(x=0), _lib.E_NULL), (dict(y=0), _lib.E_NULL), (dict(rows=0), 0), (dict(cols=0), 0), (dict(batch=0), 0)])
+    (dict(x=0), _lib.E_NULL), (dict(y=0), _lib.E_NULL), (dict(rows=0), 0), (dict(cols=0), 0), (dict(batch=0), 0),
+    (dict(rows=(1 << 30) + 1, ldx=1 << 31, ldy=1 << 31), _lib.E_TOO_LARGE)])
 def test_newton_schulz_refusals(lib, kw, status):
     assert lib.blb200_newton_schulz(ns_desc(**kw), None, 0, None) == status
 

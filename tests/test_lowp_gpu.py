@@ -12,6 +12,10 @@ newton_schulz  in the 2-norm (Frobenius) against 64 bits, by emulations in 64 bi
              of one term per stored matrix, 3 steps of them.  A store's true error is at most sqrt(3) times the uniform
              one's root mean square, and n terms of mean squares e_j^2 add up to at most sqrt(n) sqrt(sum e_j^2)
              (Cauchy-Schwarz), when all of them point the same way, as they can in a 1 x 1 matrix: sqrt(3 steps) sqrt(3) r."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -255,19 +259,19 @@ def test_refusals_of_the_python_layer(bl):
 
 
 # ---- newton_schulz ----------------------------------------------------------------------------------------------------------
-def newton_schulz_reference(g, steps, sets, eps, disturb=0.0, seed=0):
+def newton_schulz_reference(g, steps, sets, eps, disturb=0.0, seed=0, device="cpu"):
     """64-bit form on (batch, cols, rows); `disturb`: relative size of the error of every stored matrix."""
-    noise = gen(seed)
+    noise = torch.Generator(device=device).manual_seed(seed)
 
     def stored(m):
         if disturb == 0:
             return m
-        return m * (1 + disturb * (2 * torch.rand(m.shape, generator=noise, dtype=torch.float64) - 1))
+        return m * (1 + disturb * (2 * torch.rand(m.shape, generator=noise, dtype=torch.float64, device=device) - 1))
 
-    x = g.double().cpu()
+    x = g.to(device).double()
     x = stored(x / (x.flatten(1).norm(dim=1)[:, None, None] + eps))
     if x.shape[1] > x.shape[2]:
-        return newton_schulz_reference(g.transpose(1, 2), steps, sets, eps, disturb, seed).transpose(1, 2)
+        return newton_schulz_reference(g.transpose(1, 2), steps, sets, eps, disturb, seed, device).transpose(1, 2)
     for i in range(steps):
         a, b, c = sets[i % len(sets)]
         s = stored(x @ x.transpose(1, 2))
@@ -275,15 +279,15 @@ def newton_schulz_reference(g, steps, sets, eps, disturb=0.0, seed=0):
     return x
 
 
-def newton_schulz_check(got, g, kind, steps=5, sets=(QUINTIC,), eps=1e-7):
-    want = newton_schulz_reference(g, steps, sets, eps)
+def newton_schulz_check(got, g, kind, steps=5, sets=(QUINTIC,), eps=1e-7, device="cpu"):
+    want = newton_schulz_reference(g, steps, sets, eps, device=device)
     p, q = sorted(g.shape[1:])
     one_store = 2.0 ** -11 if kind == "bf16" else 2.0 ** -22 + 3 * (q / 16 + 1) * 2.0 ** -24
-    errors = torch.stack([newton_schulz_reference(g, steps, sets, eps, one_store, seed=p + q + i) - want for i in range(8)])
+    errors = torch.stack([newton_schulz_reference(g, steps, sets, eps, one_store, p + q + i, device) - want for i in range(8)])
     rms = errors.square().sum((2, 3)).mean(0).sqrt()
     for i in range(g.shape[0]):
         allowed = (9 * steps) ** 0.5 * float(rms[i]) + HALF_STEP[kind] * float(want[i].norm())
-        off = float((got[i].double().cpu() - want[i]).norm())
+        off = float((got[i].to(device).double() - want[i]).norm())
         assert off <= allowed, (i, off, allowed, float(want[i].norm()), bl_name())
 
 
@@ -308,6 +312,26 @@ def test_newton_schulz(bl, kind, batch, cols, rows):
         assert torch.equal(view.cpu(), g), "the input was written"
         out.fill_(7)
         assert bool((back == 7).all()), "padding was written"
+
+
+@pytest.mark.parametrize("kind,batch,cols,rows", [("bf16", 1, 1900, 2304), ("bf16", 2, 2111, 1700), ("f16", 1, 1100, 1900), ("f32", 1, 1500, 1333),
+                                                  ("f32", 3, 260, 1031), ("bf16", 9, 515, 1030), ("f16", 5, 700, 300)])
+def test_newton_schulz_many_tiles(bl, kind, batch, cols, rows):
+    """Pairs of CTAs, several rounds of tiles, and tiles split over clusters; the 64-bit form runs on the GPU too."""
+    g = update_like(batch, cols, rows, cols + rows, kind)
+    newton_schulz_check(bl.newton_schulz(g.cuda()), g, kind, device="cuda")
+
+
+def test_newton_schulz_layouts_of_batches(bl):
+    g = update_like(1, 40, 72, 2, "f32")
+    y = bl.newton_schulz(g.cuda().expand(3, 40, 72))                     # one matrix for every item
+    assert torch.equal(y[0], y[1]) and torch.equal(y[0], y[2])
+    newton_schulz_check(y[:1], g, "f32")
+    many = update_like(3, 150, 144, 5, "bf16").cuda()
+    side_by_side = torch.full((150, 3, 144), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = side_by_side.permute(1, 0, 2)                                  # items interleaved inside the leading dimension
+    bl.newton_schulz(many, out)
+    assert torch.equal(out, bl.newton_schulz(many))
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -423,3 +447,54 @@ def test_two_streams_at_once(bl):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
+def test_another_stream_and_its_own_scratch(bl):
+    g, x = update_like(1, 300, 200, 1, "f32").cuda(), torch.randn(9, 300, generator=gen(2)).cuda()
+    w = torch.randint(-127, 128, (70, 300), generator=gen(3), dtype=torch.int8).cuda()
+    want_y, (want_q, want_s) = bl.newton_schulz(g), bl.quantize_i8(x)
+    want_c = bl.gemm_i8(w, want_q, torch.empty(9, 70, device="cuda"), None, want_s)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    y, q, s, c = torch.zeros_like(want_y), torch.zeros_like(want_q), torch.zeros_like(want_s), torch.zeros_like(want_c)
+    torch.cuda.synchronize()
+    bl.newton_schulz(g, y, stream=side.cuda_stream)
+    bl.quantize_i8(x, q, s, stream=side.cuda_stream)
+    bl.gemm_i8(w, q, c, None, s, stream=side.cuda_stream)
+    side.synchronize()
+    for got, want in ((y, want_y), (q, want_q), (s, want_s), (c, want_c)):
+        assert torch.equal(got, want)
+
+
+FIRST_CALLS_IN_A_CAPTURE = """
+import torch, batchlas_b200 as bl
+gs = [torch.randn(2, 300, 260, device="cuda"), torch.randn(3, 64, 50, device="cuda").bfloat16()]
+ys = [torch.zeros_like(g) for g in gs]
+x = torch.randn(40, 512, device="cuda")
+w = torch.randint(-127, 128, (96, 512), device="cuda", dtype=torch.int8)
+c = torch.zeros(40, 96, device="cuda")
+torch.cuda.synchronize()
+graphs = []
+for i in range(2):                      # two graphs, each with scratch of its own
+    graphs.append(torch.cuda.CUDAGraph())
+    with torch.cuda.graph(graphs[-1]):
+        bl.newton_schulz(gs[i], ys[i])
+        q, s = bl.quantize_i8(x)
+        bl.gemm_i8(w, q, c, None, s)
+for _ in range(3):
+    for graph in graphs:
+        graph.replay()
+torch.cuda.synchronize()
+for g, y in zip(gs, ys):
+    assert torch.equal(bl.newton_schulz(g), y)
+q, s = bl.quantize_i8(x)
+assert torch.equal(bl.gemm_i8(w, q, torch.zeros_like(c), None, s), c) and float(c.abs().sum()) > 0
+assert bl.device_status() == 0
+print("replayed")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture(bl):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", FIRST_CALLS_IN_A_CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "replayed" in out.stdout, out.stdout[-2000:] + out.stderr[-2000:]
