@@ -1,5 +1,5 @@
 // Quantises every column of a batch of k x cols matrices to 8-bit integers with one scale per column:
-// scale = fl32(max |x| / 127), q = rne(fl32(x / scale)) clamped to +-127.
+// scale = fl32(max |x| * fl32(1 / 127)), q = rne(fl32(x / scale)) clamped to +-127.
 // Infinity and NaN travel through the maxima into the scale.
 #include <type_traits>
 
@@ -23,7 +23,7 @@ struct QuantizeParams {
 //   Half types: y = 127 x / max, and 2 y - odd is a multiple of 1 / (the mantissa of max): unless it is zero, y is further
 //   than y / (127 * 2047) = 3.8e-6 y from the halfway point, more than the errors together.  It is zero where 254 x = odd max:
 //   127 being prime, for y = 63.5 (half the largest value, one element in a thousand), or where max is a multiple of 127, which
-//   shows in an exact scale (one column in a hundred; divided).  So inv is moved by the last place or two that make 63.5
+//   shows in an exact quotient (one column in a hundred; divided).  So inv is moved by the few last places that make 63.5
 //   come out as the division has it, and nothing is left to check.
 //   float: |d| = |x * inv - r| within 2^-14 of one half is divided after all (one element in ten thousand).
 // Columns whose scale is so small that it or its reciprocal lose bits divide always.
@@ -33,14 +33,14 @@ struct Quantiser {
   float scale, inv;
   bool usable, divide;
   __device__ explicit Quantiser(float top) {
-    scale = __fdiv_rn(top, 127.f);
+    scale = top * (1.f / 127.f);
     usable = scale > 0.f && top < __int_as_float(0x7f800000);
-    divide = scale < 1e-36f || (HALF && fmaf(scale, 127.f, -top) == 0.f);
+    divide = scale < 1e-36f || (HALF && fmaf(__fdiv_rn(top, 127.f), 127.f, -top) == 0.f);
     inv = usable && !divide ? __frcp_rn(scale) : 0.f;
     if (HALF && usable && !divide) {
       const int want = exact(0.5f * top);
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const int got = __float_as_int(fmaf(0.5f * top, inv, kShift)) - __float_as_int(kShift);
         inv = __int_as_float(__float_as_int(inv) + (got < want ? 1 : got > want ? -1 : 0));
       }

@@ -84,7 +84,8 @@ def _scales(where, s, batch, size, shared=True):
 
 
 def quantize_i8(X, Q=None, scale=None, stream=None):
-    """Quantises every column of X: ``scale = max|x| / 127``, ``Q = round(x / scale)``, halves to even.  Q (int8, the
+    """Quantises every column of X: ``scale = max|x| * float32(1 / 127)``, ``Q = round(x / scale)``, halves to
+    even.  Q (int8, the
     shape of X) and scale (float32, one per column) are made when they are not given; returns both.  Asynchronous."""
     if Q is None:
         Q = torch.empty(X.shape, dtype=torch.int8, device=X.device)

@@ -58,7 +58,7 @@ void QuantiseAndMultiply(Queue& ctx) {
     for (int j = 0; j < m; ++j) {
       float top = 0;
       for (int l = 0; l < k; ++l) top = std::max(top, std::fabs(W[((size_t)b * m + j) * k + l]));
-      CHECK(sw[b * m + j] == top / 127.f);
+      CHECK(sw[b * m + j] == top * (1.f / 127.f));
       for (int l = 0; l < k; ++l)
         CHECK((float)Wq[((size_t)b * m + j) * k + l] == std::nearbyint(W[((size_t)b * m + j) * k + l] / sw[b * m + j]));
     }

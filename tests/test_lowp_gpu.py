@@ -57,7 +57,7 @@ def placed(x, pad=0, gap=0, offset=0, fill=7):
 def quantize_reference(x):
     """x: float32 numpy (batch, cols, k)."""
     top = np.max(np.abs(x), axis=-1) if x.shape[-1] else np.zeros(x.shape[:-1], np.float32)
-    scale = (top / np.float32(127)).astype(np.float32)
+    scale = (top * (np.float32(1) / np.float32(127))).astype(np.float32)
     usable = (scale > 0) & np.isfinite(scale)
     with np.errstate(all="ignore"):
         q = np.rint((x / np.where(usable, scale, np.float32(1))[..., None]).astype(np.float32))
