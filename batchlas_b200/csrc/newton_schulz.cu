@@ -388,7 +388,7 @@ Layout layout_of(const blb200_newton_schulz_desc* d) {
 
 // Small matrices need none, but are given some like the others, so that a caller has one rule.
 size_t workspace_need(const blb200_newton_schulz_desc* d) {
-  return newton_schulz_small_supported(d->rows, d->cols) ? 256 : layout_of(d).total;
+  return newton_schulz_small_supported(d->rows, d->cols, d->batch, d->ftype) ? 256 : layout_of(d).total;
 }
 
 Plan plan_of(const blb200_newton_schulz_desc* d) {
@@ -473,7 +473,7 @@ extern "C" int blb200_newton_schulz(const blb200_newton_schulz_desc* d, void* wo
   if (!workspace) return BLB200_E_NULL;
   if (workspace_bytes < workspace_need(d) || reinterpret_cast<uintptr_t>(workspace) % 256) return BLB200_E_SHAPE;
   cudaStream_t stream = (cudaStream_t)cuda_stream;
-  if (newton_schulz_small_supported(d->rows, d->cols)) {
+  if (newton_schulz_small_supported(d->rows, d->cols, d->batch, d->ftype)) {
     const Matrices g{const_cast<void*>(d->x), d->rows, d->cols, d->batch, d->ldx, d->stride_x};
     return launch_newton_schulz_small(g, Matrices{d->y, d->rows, d->cols, d->batch, d->ldy, d->stride_y}, d->ftype, plan_of(d), stream);
   }

@@ -301,7 +301,9 @@ def update_like(batch, cols, rows, seed, kind, size=1e-3):
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("batch,cols,rows", [(1, 1, 1), (2, 1, 40), (2, 40, 1), (3, 7, 5), (2, 16, 16), (1, 33, 65), (5, 64, 64),
                                              (2, 128, 128), (1, 100, 128), (2, 128, 250), (1, 129, 127), (1, 64, 1000), (1, 1000, 64),
-                                             (2, 200, 300), (1, 300, 200), (1, 385, 256), (1, 256, 512), (2, 520, 513)])
+                                             (2, 200, 300), (1, 300, 200), (1, 385, 256), (1, 256, 512), (2, 520, 513),
+                                             (3, 128, 512), (1, 300, 100), (2, 1000, 120), (1, 77, 1030), (2, 2048, 30), (1, 128, 1500),
+                                             (1, 100, 4096), (1, 3000, 128)])
 def test_newton_schulz(bl, kind, batch, cols, rows):
     g = update_like(batch, cols, rows, cols + rows, kind)
     for pad, gap, offset in [(0, 0, 0), (3, 5, 1)]:
@@ -315,7 +317,8 @@ def test_newton_schulz(bl, kind, batch, cols, rows):
 
 
 @pytest.mark.parametrize("kind,batch,cols,rows", [("bf16", 1, 1900, 2304), ("bf16", 2, 2111, 1700), ("f16", 1, 1100, 1900), ("f32", 1, 1500, 1333),
-                                                  ("f32", 3, 260, 1031), ("bf16", 9, 515, 1030), ("f16", 5, 700, 300)])
+                                                  ("f32", 3, 260, 1031), ("bf16", 9, 515, 1030), ("f16", 5, 700, 300),
+                                                  ("f32", 40, 128, 1000), ("f16", 30, 1030, 128), ("bf16", 300, 50, 40)])
 def test_newton_schulz_many_tiles(bl, kind, batch, cols, rows):
     """Pairs of CTAs, several rounds of tiles, and tiles split over clusters; the 64-bit form runs on the GPU too."""
     g = update_like(batch, cols, rows, cols + rows, kind)
