@@ -7,7 +7,7 @@
 // 128-byte swizzle: read as rows of q that is the K-major operand of X X^T, and read as rows of 64 q per p it is the
 // MN-major operand of B X, so it is never transposed.  S and B share one place: both S and X are only overwritten, element by
 // element by the thread that read them, after the product that uses them.  Scales and pairs of halves as in newton_schulz.cu
-// (at most 48 additions per sum here, so no partial sums).
+// (at most 32 additions to a sum of full size here, so no partial sums).
 //
 // In a cluster each CTA holds 64 QB columns of X.  X X^T is then a sum over the CTAs: each sends the rows of its part to the CTA that
 // owns them (128 / CL rows each), which adds them up in rank order and writes its rows of S to every CTA; the rest of a step
@@ -144,16 +144,19 @@ __global__ void __launch_bounds__(kThreads, PLANES == 1 && QB == 2 ? 2 : 1) newt
       const uint32_t d = tmem + n0;
       const uint32_t idesc = umma_idesc(false, false, b_mn, 128, n);
       const uint32_t lead = b_mn ? 16384 : 16;
+      auto at = [&](const unsigned char* p, int k, bool mn) {
+        return umma_desc(smem_u32(p) + (mn ? k * 2048 : (k >> 2) * 16384 + (k & 3) * 32), mn ? lead : 16, 1024);
+      };
+      // the small products first: an addition drops what lies below the last place of the sum that it adds to
+      if constexpr (PLANES == 2) {
 #pragma unroll 4
-      for (int k = 0; k < k_steps; ++k) {
-        const uint32_t step = (k >> 2) * 16384 + (k & 3) * 32, step_b = b_mn ? k * 2048 : step;
-        const uint64_t da = umma_desc(smem_u32(a) + step, 16, 1024), db = umma_desc(smem_u32(b) + step_b, lead, 1024);
-        umma<1, false>(d, da, db, idesc, k > 0);
-        if constexpr (PLANES == 2) {
-          umma<1, false>(d, da, umma_desc(smem_u32(b) + plane_b + step_b, lead, 1024), idesc, true);
-          umma<1, false>(d, umma_desc(smem_u32(a) + plane_a + step, 16, 1024), db, idesc, true);
+        for (int k = 0; k < k_steps; ++k) {
+          umma<1, false>(d, at(a, k, false), at(b + plane_b, k, b_mn), idesc, k > 0);
+          umma<1, false>(d, at(a + plane_a, k, false), at(b, k, b_mn), idesc, true);
         }
       }
+#pragma unroll 4
+      for (int k = 0; k < k_steps; ++k) umma<1, false>(d, at(a, k, false), at(b, k, b_mn), idesc, PLANES == 2 || k > 0);
     }
     if (threadIdx.x == 0) umma_commit<1>(&ready);
     __syncwarp();

@@ -316,17 +316,17 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           // 32 bytes of k per instruction: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major block
           constexpr uint32_t kAStep = C::A_MN ? 2048 : 32, kBStep = C::B_MN ? 2048 : 32;
           constexpr uint32_t kALead = C::A_MN ? 8192 : 16, kBLead = C::B_MN ? 8192 : 16;
+          auto desc_a = [&](int plane, int ks) { return umma_desc(a + plane * C::kABytes + ks * kAStep, kALead, 1024); };
+          auto desc_b = [&](int plane, int ks) { return umma_desc(b + plane * C::kBBytes + ks * kBStep, kBLead, 1024); };
+          if constexpr (C::PLANES == 2) {  // the small products first, while the sum that they are added to is small as well
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint64_t da = umma_desc(a + ks * kAStep, kALead, 1024), db = umma_desc(b + ks * kBStep, kBLead, 1024);
-            umma<G, C::I8>(d, da, db, idesc, !begins || ks > 0);
-            if constexpr (C::PLANES == 2) {
-              const uint64_t da2 = umma_desc(a + C::kABytes + ks * kAStep, kALead, 1024);
-              const uint64_t db2 = umma_desc(b + C::kBBytes + ks * kBStep, kBLead, 1024);
-              umma<G, C::I8>(d, da, db2, idesc, true);
-              umma<G, C::I8>(d, da2, db, idesc, true);
+            for (int ks = 0; ks < 4; ++ks) {
+              umma<G, C::I8>(d, desc_a(0, ks), desc_b(1, ks), idesc, !begins || ks > 0);
+              umma<G, C::I8>(d, desc_a(1, ks), desc_b(0, ks), idesc, true);
             }
           }
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) umma<G, C::I8>(d, desc_a(0, ks), desc_b(0, ks), idesc, C::PLANES == 2 || !begins || ks > 0);
           umma_commit<G>(&empty[slot]);
           if (++slot == S) {
             slot = 0;
