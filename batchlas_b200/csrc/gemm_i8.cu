@@ -52,8 +52,9 @@ template <bool WHOLE>
 __device__ __forceinline__ uint4 load16(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
   if (WHOLE && valid >= 16) return *reinterpret_cast<const uint4*>(src);
   if (valid <= 0) return make_uint4(0, 0, 0, 0);
-  const Words16 w = load16_words(src, valid, lo, hi);
-  return w.edge ? load16_bytes(src, valid) : valid < 16 ? first_bytes(w.v, valid) : w.v;
+  Words16 w;
+  w.load(src, valid, lo, hi);
+  return w.edge ? load16_bytes(src, valid) : valid < 16 ? first_bytes(w.value(src), valid) : w.value(src);
 }
 
 // WHOLE: both operands' columns start on 16-byte boundaries.

@@ -307,7 +307,7 @@ int launch_product(Maps& maps, const Operands& o, const typename Epilogue::Param
 
 // Tiles of 256 rows on CTA pairs (256 columns wide, for pairs of halves 128), of 128 x 128 on single CTAs, or of 128 x 128
 // with k split over two or four CTAs: whichever should take the least time, in units of about 0.3 us: per 64 k a tile of 128 x
-// 128 takes one (pairs of halves: two and a half), a pair's takes 1.3 (2.5), a tile's start and end 12, an exchange 6.
+// 128 takes one (pairs of halves: two and a half), a pair's takes 1.3 (2.5), a tile's start and end 12, an exchange 3.
 template <bool A_MN, bool B_MN, int PLANES, class Epilogue>
 int product(Maps& maps, const Operands& o, const typename Epilogue::Params& ep, cudaStream_t stream) {
   constexpr int kPairN = PLANES == 2 ? 128 : 256;

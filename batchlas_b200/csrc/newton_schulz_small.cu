@@ -7,7 +7,8 @@
 // 128-byte swizzle: read as rows of q that is the K-major operand of X X^T, and read as rows of 64 q per p it is the
 // MN-major operand of B X, so it is never transposed.  S and B share one place: both S and X are only overwritten, element by
 // element by the thread that read them, after the product that uses them.  Scales and pairs of halves as in newton_schulz.cu
-// (at most 32 additions to a sum of full size here, so no partial sums).
+// (at most 32 additions to a sum of full size here, so no partial sums), but that bfloat16 keeps B as a pair as well: with few rows its
+// rounding weighs most (six steps on 128 x 128: 2.1e-3 of the result in all instead of 2.5e-3), and here the second product is free.
 //
 // In a cluster each CTA holds 64 QB columns of X.  X X^T is then a sum over the CTAs: each sends the rows of its part to the CTA that
 // owns them (128 / CL rows each), which adds them up in rank order and writes its rows of S to every CTA; the rest of a step
@@ -29,7 +30,8 @@ constexpr int kThreads = 512, kParts = kThreads / 128;  // warps per quarter of 
 template <int PLANES, int QB, int CL>
 struct SmallMemory {
   static constexpr int kX = QB * 128 * 128, kS = 2 * 128 * 128;  // bytes of one plane
-  static constexpr int kShared = CL > 1 && PLANES * kS < 65536 ? 65536 : PLANES * kS;  // S and B, or the parts of 128 x 128 sums
+  static constexpr int kShared = 2 * kS;  // S and then B, which has two planes always, or the parts of 128 x 128 float sums
+  static_assert(kShared == 128 * 128 * 4, "");
   static constexpr size_t kBytes = 1024 + (size_t)PLANES * kX + kShared;
   static constexpr int kColumns = QB * 64 < 128 ? 128 : QB * 64;
 };
@@ -137,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, PLANES == 1 && QB == 2 ? 2 : 1) newt
   bool ok = true;
   // One product by thread 0: A from `a` (K-major), B from `b`, K = 16 k_steps, N = n (a multiple of 256 as several instructions); all
   // threads return when it is done.
-  auto product = [&](const unsigned char* a, int plane_a, const unsigned char* b, int plane_b, bool b_mn, int k_steps, int n_all) {
+  auto product = [&](const unsigned char* a, int plane_a, const unsigned char* b, int plane_b, bool b_mn, int k_steps, int n_all, bool a_low) {
     if (!ok) return;
     const int n = min(n_all, 256);
     for (int n0 = 0; n0 < n_all && threadIdx.x == 0; n0 += n, b += 4 * 16384) {
@@ -155,8 +157,12 @@ __global__ void __launch_bounds__(kThreads, PLANES == 1 && QB == 2 ? 2 : 1) newt
           umma<1, false>(d, at(a + plane_a, k, false), at(b, k, b_mn), idesc, true);
         }
       }
+      if (PLANES == 1 && a_low) {
 #pragma unroll 4
-      for (int k = 0; k < k_steps; ++k) umma<1, false>(d, at(a, k, false), at(b, k, b_mn), idesc, PLANES == 2 || k > 0);
+        for (int k = 0; k < k_steps; ++k) umma<1, false>(d, at(a + plane_a, k, false), at(b, k, b_mn), idesc, k > 0);
+      }
+#pragma unroll 4
+      for (int k = 0; k < k_steps; ++k) umma<1, false>(d, at(a, k, false), at(b, k, b_mn), idesc, PLANES == 2 || a_low || k > 0);
     }
     if (threadIdx.x == 0) umma_commit<1>(&ready);
     __syncwarp();
@@ -192,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, PLANES == 1 && QB == 2 ? 2 : 1) newt
       }
     }
   };
-  auto epilogue = [&](unsigned char* at, int plane, int columns, float2 f, bool has_old) {
+  auto epilogue = [&](unsigned char* at, int plane, int columns, float2 f, bool has_old, bool low) {
 #pragma unroll 1
     for (int c = part * (columns / kParts); c < (part + 1) * (columns / kParts); c += 16) {
       float r[16];
@@ -205,10 +211,10 @@ __global__ void __launch_bounds__(kThreads, PLANES == 1 && QB == 2 ? 2 : 1) newt
           const float r0 = r[8 * h + 2 * i], r1 = r[8 * h + 2 * i + 1];
           const __half h0 = __float2half_rn(r0), h1 = __float2half_rn(r1);
           hi[i] = pack_halves(h0, h1);
-          if constexpr (PLANES == 2) lo[i] = pack_halves(__float2half_rn(r0 - __half2float(h0)), __float2half_rn(r1 - __half2float(h1)));
+          lo[i] = pack_halves(__float2half_rn(r0 - __half2float(h0)), __float2half_rn(r1 - __half2float(h1)));
         }
         *reinterpret_cast<uint4*>(at + chunk_at(row, (c >> 3) + h)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(at + plane + chunk_at(row, (c >> 3) + h)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (PLANES == 2 || low) *reinterpret_cast<uint4*>(at + plane + chunk_at(row, (c >> 3) + h)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     tc_fence_before();
@@ -281,14 +287,14 @@ __global__ void __launch_bounds__(kThreads, PLANES == 1 && QB == 2 ? 2 : 1) newt
 #pragma unroll 1
   for (int i = 0; i < plan.steps; ++i) {
     const float2* f = factors + 3 * i;
-    product(x, M::kX, x, M::kX, false, QB * 4, 128);
+    product(x, M::kX, x, M::kX, false, QB * 4, 128, false);
     if constexpr (CL > 1) share_gram(f[0].x);
-    else epilogue(sb, M::kS, 128, f[0], false);
-    product(sb, M::kS, sb, M::kS, false, 8, 128);
-    epilogue(sb, M::kS, 128, f[1], true);
-    product(sb, M::kS, x, M::kX, true, 8, QB * 64);
+    else epilogue(sb, M::kS, 128, f[0], false, false);
+    product(sb, M::kS, sb, M::kS, false, 8, 128, false);
+    epilogue(sb, M::kS, 128, f[1], true, true);
+    product(sb, M::kS, x, M::kX, true, 8, QB * 64, true);
     if (i + 1 < plan.steps) {
-      epilogue(x, M::kX, QB * 64, f[2], true);
+      epilogue(x, M::kX, QB * 64, f[2], true, false);
     } else {
       T* out = (T*)y.p + item * y.stride;
       const int p = wide ? y.rows : y.cols, q = wide ? y.cols : y.rows;

@@ -20,7 +20,7 @@
 // distributed shared memory (the idle stages), each CTA adding up, in rank order, what it stores.  For calls whose
 // tiles would leave most SMs without work.
 // PLAIN: the operands are not on 16-byte boundaries, so the eight epilogue warps fetch the stages themselves, as aligned words
-// shifted together and written where the swizzle puts them (777 x 4099 x 1003 with its quantisation 35 us; a row at a time, one word
+// shifted together and written where the swizzle puts them (777 x 4099 x 1003 with its quantisation 37 us; a row at a time, one word
 // per lane and the neighbour's by a shuffle, measured 52).
 //
 // Measured: 8192^3 8-bit 380 us = 2.9 POP/s, where the MMAs alone, without fetches and stores, take 345 and the fetches alone 215;
@@ -134,27 +134,34 @@ struct PlainOperands {
   long long lda, ldb, sa, sb;
 };
 
-// 16 bytes at `src` (any alignment) of which the first `valid` exist, the rest zero.  [lo, hi) is the operand.  The five aligned
-// words around them are read and shifted together, without branches, so that many such loads can be in flight; where
-// one of them reaches over an end of the operand, `edge` says so and load16_bytes has to do it.
+// 16 bytes at `src` (any alignment) of which the first `valid` exist, the rest zero.  [lo, hi) is the operand.  The two aligned
+// 16-byte pieces around them are read without branches, so that many such loads can be in flight, and shifted together when
+// they are used; where one of them reaches over an end of the operand, `edge` says so and load16_bytes has to do it.
 struct Words16 {
-  uint4 v;
+  uint4 p, q;
   bool edge;
-};
-__device__ __forceinline__ Words16 load16_words(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
-  const int off = (int)(reinterpret_cast<uintptr_t>(src) & 3u);
-  const int8_t* base = src - off;
-  const bool exists = valid > 0, inside = base >= lo && base + 20 <= hi;
-  uint32_t x[5];
-#pragma unroll
-  for (int j = 0; j < 5; ++j) {
-    x[j] = 0;
-    if (exists && inside) x[j] = reinterpret_cast<const uint32_t*>(base)[j];
+  __device__ __forceinline__ void load(const int8_t* src, int valid, const int8_t* lo, const int8_t* hi) {
+    const int8_t* base = src - (reinterpret_cast<uintptr_t>(src) & 15u);
+    const bool exists = valid > 0, inside = base >= lo && base + 32 <= hi;
+    p = q = make_uint4(0, 0, 0, 0);
+    if (exists && inside) {
+      p = *reinterpret_cast<const uint4*>(base);
+      q = *reinterpret_cast<const uint4*>(base + 16);
+    }
+    edge = exists && !inside;
   }
-  return Words16{make_uint4(__funnelshift_r(x[0], x[1], off * 8), __funnelshift_r(x[1], x[2], off * 8), __funnelshift_r(x[2], x[3], off * 8),
-                            __funnelshift_r(x[3], x[4], off * 8)),
-                 exists && !inside};
-}
+  __device__ __forceinline__ uint4 value(const int8_t* src) const {
+    const int off = (int)(reinterpret_cast<uintptr_t>(src) & 15u), sh = (off & 3) * 8;
+    const uint32_t x[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+    uint32_t t[6], u[5];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) t[i] = off & 8 ? x[i + 2] : x[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) u[i] = off & 4 ? t[i + 1] : t[i];
+    return make_uint4(__funnelshift_r(u[0], u[1], sh), __funnelshift_r(u[1], u[2], sh), __funnelshift_r(u[2], u[3], sh),
+                      __funnelshift_r(u[3], u[4], sh));
+  }
+};
 __device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >= 4 ? w : n <= 0 ? 0u : w & (0xffffffffu >> (8 * (4 - n))); }
 __device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
   return make_uint4(first_bytes(v.x, n), first_bytes(v.y, n - 4), first_bytes(v.z, n - 8), first_bytes(v.w, n - 12));
@@ -356,7 +363,9 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     uint32_t done = 0, tiles_done = 0;
     auto acquire = [&]() {
       const int acc = (int)(done & 1);
-      const bool got = mbar_wait(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc);
+      // the one wait that lasts as long as a tile's whole sum: its limit grows with the number of k blocks
+      const bool got = mbar_wait_limit(&acc_full[acc], (uint32_t)((done >> 1) & 1), wait_code + kUmmaWaitAcc,
+                                       kSpinLimit * (uint32_t)min(256, 1 + (k_blocks >> 12)));
       tc_fence_after();
       return (bool)__all_sync(0xffffffffu, got);
     };
@@ -396,37 +405,51 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const int8_t* b = po.b + tile.item * po.sb;
         const int8_t* a_end = a + (long long)(s.m - 1) * po.lda + s.k;
         const int8_t* b_end = b + (long long)(s.n - 1) * po.ldb + s.k;
-        const int tid = (int)threadIdx.x - 64;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty));
-          if (!ok) break;
-          unsigned char* stage = smem + (size_t)slot * C::kStageBytes;
-          const int chunk = tid & 7, kk = (kb_begin + kb) * 128 + chunk * 16, valid = s.k - kk;
-          constexpr int kRows = 128 + C::kBRows, kEach = kRows / 32;
-          // rows (tid >> 3) + 32 i: those of A (i < 4), then those of B; both start on a multiple of eight rows
-          const int r0 = tid >> 3, ma = tile.tm * 128 + r0, nb = tile.tn * C::BN + r0;
-          const int8_t* at_a = a + (long long)ma * po.lda + kk;
-          const int8_t* at_b = b + (long long)nb * po.ldb + kk;
-          unsigned char* to = stage + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
-          auto bytes_of = [&](int i) { return (i < 4 ? ma + 32 * i < s.m : nb + 32 * (i - 4) < s.n) ? valid : 0; };
-          auto source = [&](int i) { return i < 4 ? at_a + (long long)(32 * i) * po.lda : at_b + (long long)(32 * (i - 4)) * po.ldb; };
-          Words16 v[kEach];
+        // Sixteen bytes of every 32nd row per thread: those of A (i < 4), then those of B; both start on a multiple of eight rows.
+        // One half of them is on its way while the other is shifted and stored.
+        constexpr int kEach = (128 + C::kBRows) / 32;
+        const int r0 = ((int)threadIdx.x - 64) >> 3, chunk = threadIdx.x & 7, ma = tile.tm * 128 + r0, nb = tile.tn * C::BN + r0;
+        const int8_t* at_a = a + (long long)ma * po.lda + chunk * 16;
+        const int8_t* at_b = b + (long long)nb * po.ldb + chunk * 16;
+        auto k_of = [&](int kb) { return (kb_begin + kb) * 128; };
+        auto bytes_of = [&](int i, int kb) { return (i < 4 ? ma + 32 * i < s.m : nb + 32 * (i - 4) < s.n) ? s.k - k_of(kb) - chunk * 16 : 0; };
+        auto source = [&](int i, int kb) { return (i < 4 ? at_a + (long long)(32 * i) * po.lda : at_b + (long long)(32 * (i - 4)) * po.ldb) + k_of(kb); };
+        constexpr int kHalf = kEach / 2;
+        auto load = [&](int part, Words16 (&v)[kHalf], int kb) {
+#pragma unroll
+          for (int h = 0; h < kHalf; ++h) {
+            const int i = part * kHalf + h;
+            v[h].load(source(i, kb), bytes_of(i, kb), i < 4 ? a : b, i < 4 ? a_end : b_end);
+          }
+        };
+        auto store = [&](int part, const Words16 (&v)[kHalf], int kb) {
+          unsigned char* to = smem + (size_t)slot * C::kStageBytes + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
+          const int valid = s.k - k_of(kb) - chunk * 16;
           bool edge = false;
 #pragma unroll
-          for (int i = 0; i < kEach; ++i) {
-            v[i] = load16_words(source(i), bytes_of(i), i < 4 ? a : b, i < 4 ? a_end : b_end);
-            edge |= v[i].edge;
+          for (int h = 0; h < kHalf; ++h) {
+            const int i = part * kHalf + h;
+            uint4 w = v[h].value(source(i, kb));
+            if (valid < 16) w = first_bytes(w, valid);
+            *reinterpret_cast<uint4*>(to + i * 32 * 128) = w;
+            edge |= v[h].edge;
           }
-          if (valid < 16) {
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) v[i].v = first_bytes(v[i].v, valid);
-          }
-#pragma unroll
-          for (int i = 0; i < kEach; ++i) *reinterpret_cast<uint4*>(to + i * 32 * 128) = v[i].v;
           if (edge) {
 #pragma unroll 1
-            for (int i = 0; i < kEach; ++i) *reinterpret_cast<uint4*>(to + i * 32 * 128) = load16_bytes(source(i), bytes_of(i));
+            for (int i = part * kHalf; i < (part + 1) * kHalf; ++i)
+              *reinterpret_cast<uint4*>(to + i * 32 * 128) = load16_bytes(source(i, kb), bytes_of(i, kb));
           }
+        };
+        Words16 v0[kHalf], v1[kHalf];
+        load(0, v0, 0);
+#pragma unroll 1
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          load(1, v1, kb);
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], (round & 1) ^ 1, wait_code + kUmmaWaitEmpty));
+          if (!ok) break;
+          store(0, v0, kb);
+          if (kb + 1 < k_blocks) load(0, v0, kb + 1);
+          store(1, v1, kb);
           fence_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&full[slot]);

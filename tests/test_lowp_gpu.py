@@ -379,6 +379,44 @@ def test_newton_schulz_non_finite_items_stay_apart(bl, kind, cols, rows):
     newton_schulz_check(y[[0, 3]], g[[0, 3]], kind)
 
 
+# ---- sizes past 32 bits -----------------------------------------------------------------------------------------------------
+def test_quantize_and_product_past_32_bit_offsets(bl):
+    k, cols = 40000, 60001                                  # 2.4e9 elements
+    x = torch.zeros(cols, k, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = torch.randn(3, k, generator=gen(1)).to(torch.bfloat16).cuda()
+    q, s = bl.quantize_i8(x)
+    want_q, want_s = quantize_reference(x[-3:].float().cpu().numpy())
+    assert np.array_equal(q[-3:].cpu().numpy(), want_q) and np.array_equal(s[-3:].cpu().numpy(), want_s)
+    assert not bool(s[:-3].any()) and not bool(q[:-3].any())
+    del x
+    for n in (4, 40):
+        b = torch.randint(-128, 128, (n, k), generator=gen(n), dtype=torch.int8).cuda()
+        c = bl.gemm_i8(q, b, torch.empty(n, cols, device="cuda"))
+        assert torch.equal(c[:, -3:].double(), b.double() @ q[-3:].double().T) and not bool(c[:, :-3].any())
+        odd = q.flatten()[1:1 + (cols - 1) * k].view(cols - 1, k)   # the same bytes, every column one byte later
+        c = bl.gemm_i8(odd, b, torch.empty(n, cols - 1, device="cuda"))
+        assert torch.equal(c[:, -3:].double(), b.double() @ odd[-3:].double().T) and not bool(c[:, :-3].any())
+
+
+def test_newton_schulz_past_32_bit_offsets(bl):
+    """120 x 18 000 001: the iteration is X0 times a polynomial of the 120 x 120 Gram matrix, which 64 bits give exactly enough.
+    Three steps of three stores, each off by at most 2^-11 and amplified by at most 3.9 per step that follows, and Y's half step."""
+    rows, cols, steps = 120, 18_000_001, 3
+    g = torch.empty(cols, rows, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(3))
+    gram = sum(part.double().T @ part.double() for part in g.split(2_000_000))
+    f = float(gram.trace()) ** 0.5 + 1e-7
+    one, s = torch.eye(rows, dtype=torch.float64, device="cuda"), gram / f ** 2
+    total, (a, b, c) = one, QUINTIC
+    for _ in range(steps):
+        poly = a * one + b * s + c * s @ s
+        total, s = total @ poly, poly @ s @ poly
+    y = bl.newton_schulz(g, steps=steps)
+    allowed = sum(3 * 2.0 ** -11 * 3.9 ** i for i in range(steps)) + 2.0 ** -8
+    for part in (slice(0, 1000), slice(cols // 2, cols // 2 + 1000), slice(cols - 1000, cols)):
+        want = g[part].double() / f @ total
+        assert float((y[part].double() - want).norm()) <= allowed * float(want.norm())
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------------
 def test_update_quantise_and_serve(bl):
     """A weight takes an orthogonalised update, is quantised by channel and multiplies quantised activations."""
