@@ -8,7 +8,7 @@
 // MN-major operand of B X, so it is never transposed.  S and B share one place: both S and X are only overwritten, element by
 // element by the thread that read them, after the product that uses them.  Scales and pairs of halves as in newton_schulz.cu
 // (at most 32 additions to a sum of full size here, so no partial sums), but that bfloat16 keeps B as a pair as well: with few rows its
-// rounding weighs most (six steps on 128 x 128: 2.1e-3 of the result in all instead of 2.5e-3), and here the second product is free.
+// rounding weighs most (six steps on 128 x 128: 2.1e-3 of the result in all instead of 2.5e-3, for 34 us instead of 30).
 //
 // In a cluster each CTA holds 64 QB columns of X.  X X^T is then a sum over the CTAs: each sends the rows of its part to the CTA that
 // owns them (128 / CL rows each), which adds them up in rank order and writes its rows of S to every CTA; the rest of a step
@@ -16,8 +16,8 @@
 // exchange.  A wait that runs out lets the CTA go through the remaining barriers without products.
 //
 // Bound by latency: a product, its completion, the epilogue's pass over tensor and shared memory and two barriers of the CTA take
-// about 1.1 us (4 us for a step of 128 x 128 bfloat16, 8 to 11 with a cluster's exchange), against 6 for a launch of its own:
-// 64 of 128 x 128 bfloat16 30 us (98 as products over all items), 128 x 2048 65 us (about 115).
+// about 1.5 us (5 us for a step of 128 x 128 bfloat16, 8 to 11 with a cluster's exchange), against 6 for a launch of its own:
+// 64 of 128 x 128 bfloat16 34 us (98 as products over all items), 128 x 2048 71 us (about 115).
 #include "newton_schulz.cuh"
 #include "tcgen05.cuh"
 

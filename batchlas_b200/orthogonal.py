@@ -40,8 +40,7 @@ def newton_schulz(X, Y=None, steps=5, coefficients=QUINTIC, eps=1e-7, *, workspa
 
     Y is made when it is not given and may be X.  float32 and float16 keep float accuracy throughout (every
     intermediate matrix is a pair of float16 matrices); bfloat16 keeps one float16 matrix of each, times a power of two.
-    Y is rounded once.  The scratch
-    comes from torch's caching allocator unless `workspace` (a CUDA uint8 tensor, 256-byte aligned, of at least
+    Y is rounded once.  The scratch comes from torch's caching allocator unless `workspace` (a CUDA uint8 tensor, 256-byte aligned, of at least
     :func:`newton_schulz_workspace_bytes` bytes) is given.  Asynchronous."""
     if Y is None:
         Y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
