@@ -85,6 +85,7 @@ class NewtonSchulzDesc(ctypes.Structure):
                 ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("batch", ctypes.c_int32),
                 ("ldx", ctypes.c_int64), ("ldy", ctypes.c_int64), ("stride_x", ctypes.c_int64), ("stride_y", ctypes.c_int64),
                 ("ftype", ctypes.c_int32), ("steps", ctypes.c_int32), ("coefficient_sets", ctypes.c_int32),
+                ("half_intermediates", ctypes.c_int32),
                 ("coefficients", ctypes.POINTER(ctypes.c_double)), ("eps", ctypes.c_double)]
 
 

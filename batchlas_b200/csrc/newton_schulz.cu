@@ -4,11 +4,12 @@
 // The products run on the fp16 tensor cores with float accumulation.  X, S and B are stored in half precision, each
 // times a power of two of its own that puts the largest value it can reach just below half's range: |X|_2 is known
 // from the coefficients (it starts at ||G||/(||G|| + eps) <= 1 and each step maps it through the polynomial), and no
-// entry exceeds the norm.  float inputs keep every matrix as a pair hi + lo of halves (22 bits and a sign) and
-// multiply three times, and so do float16 inputs: one half per value would leave 1.2e-3 of the result, four times
-// what float16's own rounding does.  bfloat16 inputs keep one half per value, whose half step of 2^-11 is an eighth of
-// bfloat16's (2.0e-3 of the result in all, of which bfloat16's rounding is 1.7e-3).  What the scales come to is worked out on the device, per item and step, as the
-// factors (alpha, beta) of the three products' epilogues  out = alpha * product + beta * old.
+// entry exceeds the norm.  Every matrix is kept as a pair hi + lo of halves (22 bits and a sign) and multiplied three times: one
+// half per value leaves 1.0 to 1.4e-3 of the result, five times what float16's own rounding does, and with bfloat16's, which is
+// 1.65e-3, 1.9 to 2.2e-3 in all.  Only a caller who asks for it gets that (bfloat16, half_intermediates: 4096 x 16384 4.1 ms, as
+// pairs 14.0).  No cheaper way lies between: with any one of the products' operands in single halves 0.3 to 1.0e-3 are
+// left.  What the scales come to is worked out on the device, per item and step, as the factors (alpha, beta) of the three
+// products' epilogues  out = alpha * product + beta * old.
 //
 // Layout: X keeps the caller's orientation (rows fastest), so nothing is transposed.  With rows <= cols the Gram product
 // contracts over the slow index (both operands MN-major) and the update over the fast one; with rows > cols the other
@@ -340,6 +341,7 @@ int validate_ns(const blb200_newton_schulz_desc* d) {
   if (!readable_layout(d->rows, d->ldx, d->stride_x) || !writable_layout(d->rows, d->cols, d->batch, d->ldy, d->stride_y))
     return BLB200_E_SHAPE;
   if (d->batch > 65535 || d->rows > kMaxDim || d->cols > kMaxDim) return BLB200_E_TOO_LARGE;
+  if (d->half_intermediates != 0 && (d->half_intermediates != 1 || d->ftype != BLB200_BF16)) return BLB200_E_UNSUPPORTED;
   if (d->steps < 1 || d->steps > kMaxSteps || !(d->eps >= 0.0) || !isfinite(d->eps)) return BLB200_E_UNSUPPORTED;
   if (!d->coefficients) return BLB200_E_NULL;
   if (d->coefficient_sets != 1 && d->coefficient_sets != d->steps) return BLB200_E_UNSUPPORTED;
@@ -356,6 +358,8 @@ int validate_ns(const blb200_newton_schulz_desc* d) {
   return BLB200_OK;
 }
 
+int planes_of(const blb200_newton_schulz_desc* d) { return d->half_intermediates ? 1 : 2; }
+
 struct Layout {
   int planes, p;
   long long ld_x, plane_x, ld_s, plane_s;  // elements
@@ -364,7 +368,7 @@ struct Layout {
 Layout layout_of(const blb200_newton_schulz_desc* d) {
   Layout l;
   const size_t n = d->batch;
-  l.planes = d->ftype == BLB200_BF16 ? 1 : 2;
+  l.planes = planes_of(d);
   l.p = d->rows < d->cols ? d->rows : d->cols;
   l.ld_x = ((long long)d->rows + 7) / 8 * 8;
   l.plane_x = l.ld_x * d->cols;
@@ -388,7 +392,7 @@ Layout layout_of(const blb200_newton_schulz_desc* d) {
 
 // Small matrices need none, but are given some like the others, so that a caller has one rule.
 size_t workspace_need(const blb200_newton_schulz_desc* d) {
-  return newton_schulz_small_supported(d->rows, d->cols, d->batch, d->ftype) ? 256 : layout_of(d).total;
+  return newton_schulz_small_supported(d->rows, d->cols, d->batch, planes_of(d)) ? 256 : layout_of(d).total;
 }
 
 Plan plan_of(const blb200_newton_schulz_desc* d) {
@@ -473,12 +477,13 @@ extern "C" int blb200_newton_schulz(const blb200_newton_schulz_desc* d, void* wo
   if (!workspace) return BLB200_E_NULL;
   if (workspace_bytes < workspace_need(d) || reinterpret_cast<uintptr_t>(workspace) % 256) return BLB200_E_SHAPE;
   cudaStream_t stream = (cudaStream_t)cuda_stream;
-  if (newton_schulz_small_supported(d->rows, d->cols, d->batch, d->ftype)) {
+  if (newton_schulz_small_supported(d->rows, d->cols, d->batch, planes_of(d))) {
     const Matrices g{const_cast<void*>(d->x), d->rows, d->cols, d->batch, d->ldx, d->stride_x};
-    return launch_newton_schulz_small(g, Matrices{d->y, d->rows, d->cols, d->batch, d->ldy, d->stride_y}, d->ftype, plan_of(d), stream);
+    return launch_newton_schulz_small(g, Matrices{d->y, d->rows, d->cols, d->batch, d->ldy, d->stride_y}, d->ftype, planes_of(d), plan_of(d), stream);
   }
   const Layout l = layout_of(d);
   if (d->ftype == BLB200_F32) return run<float, 2>(d, l, (char*)workspace, stream);
   if (d->ftype == BLB200_F16) return run<__half, 2>(d, l, (char*)workspace, stream);
+  if (l.planes == 2) return run<__nv_bfloat16, 2>(d, l, (char*)workspace, stream);
   return run<__nv_bfloat16, 1>(d, l, (char*)workspace, stream);
 }

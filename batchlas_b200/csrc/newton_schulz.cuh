@@ -123,8 +123,8 @@ __device__ __forceinline__ uint32_t pack_halves(__half a, __half b) {
 }
 __device__ __forceinline__ __half half_of(uint32_t pair, int which) { return __ushort_as_half((unsigned short)(pair >> (16 * which))); }
 
-// One CTA or cluster per matrix, for matrices that fit.
-bool newton_schulz_small_supported(int rows, int cols, int batch, int ftype);
-int launch_newton_schulz_small(const Matrices& g, const Matrices& y, int ftype, const Plan& plan, cudaStream_t stream);
+// One CTA or cluster per matrix, for matrices that fit; planes: halves per stored value.
+bool newton_schulz_small_supported(int rows, int cols, int batch, int planes);
+int launch_newton_schulz_small(const Matrices& g, const Matrices& y, int ftype, int planes, const Plan& plan, cudaStream_t stream);
 
 }  // namespace blb200

@@ -7,8 +7,8 @@
 // 128-byte swizzle: read as rows of q that is the K-major operand of X X^T, and read as rows of 64 q per p it is the
 // MN-major operand of B X, so it is never transposed.  S and B share one place: both S and X are only overwritten, element by
 // element by the thread that read them, after the product that uses them.  Scales and pairs of halves as in newton_schulz.cu
-// (at most 32 additions to a sum of full size here, so no partial sums), but that bfloat16 keeps B as a pair as well: with few rows its
-// rounding weighs most (six steps on 128 x 128: 2.1e-3 of the result in all instead of 2.5e-3, for 34 us instead of 30).
+// (at most 16 additions to a sum of full size here, so no partial sums).  Where the caller asks for single halves, B stays a
+// pair: with few rows its rounding weighs most (six steps on 128 x 128: 2.1e-3 of the result in all instead of 2.5e-3, for 34 us instead of 30).
 //
 // In a cluster each CTA holds 64 QB columns of X.  X X^T is then a sum over the CTAs: each sends the rows of its part to the CTA that
 // owns them (128 / CL rows each), which adds them up in rank order and writes its rows of S to every CTA; the rest of a step
@@ -401,17 +401,17 @@ int launch_by_size(const Matrices& g, const Matrices& y, const Plan& plan, cudaS
 // The shorter side in one tile and the longer one in the shared memory of a cluster.  Batches whose clusters do not all run at
 // once (about 14 of eight CTAs do, one CTA per SM) are as fast or faster as products over all items: 14 matrices of 128 x 4096 bfloat16
 // take 92 us here, and fifteen 165 as products, where sixteen would take 173 here.
-bool newton_schulz_small_supported(int rows, int cols, int batch, int ftype) {
+bool newton_schulz_small_supported(int rows, int cols, int batch, int planes) {
   const int p = rows < cols ? rows : cols, q = rows < cols ? cols : rows;
-  if (p > 128 || q > (ftype == BLB200_BF16 ? 4096 : 2048)) return false;
+  if (p > 128 || q > (planes == 1 ? 4096 : 2048)) return false;
   const int ctas = q <= 256 ? 1 : q <= 512 ? 2 : q <= 1024 ? 4 : 8;
   return ctas == 1 || (long long)batch * ctas <= 112;
 }
 
-int launch_newton_schulz_small(const Matrices& g, const Matrices& y, int ftype, const Plan& plan, cudaStream_t stream) {
+int launch_newton_schulz_small(const Matrices& g, const Matrices& y, int ftype, int planes, const Plan& plan, cudaStream_t stream) {
   if (ftype == BLB200_F32) return launch_by_size<float, 2>(g, y, plan, stream);
   if (ftype == BLB200_F16) return launch_by_size<__half, 2>(g, y, plan, stream);
-  return launch_by_size<__nv_bfloat16, 1>(g, y, plan, stream);
+  return planes == 1 ? launch_by_size<__nv_bfloat16, 1>(g, y, plan, stream) : launch_by_size<__nv_bfloat16, 2>(g, y, plan, stream);
 }
 
 int newton_schulz_small_device_status(int* out) { return read_device_status_word(out); }

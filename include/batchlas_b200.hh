@@ -1060,6 +1060,7 @@ struct NewtonSchulzOptions {
   int steps = 5;
   std::vector<double> coefficients = {3.4445, -4.7750, 2.0315};  // one triple, or one for each step
   double eps = 1e-7;
+  bool half_intermediates = false;  // bfloat16 only: faster, less exact
 };
 
 // Q and scale <- every column of X quantised.
@@ -1116,6 +1117,7 @@ inline Event newton_schulz(Queue& ctx, const MatrixView<T, MatrixFormat::Dense>&
   d.steps = o.steps; d.coefficient_sets = (int)(o.coefficients.size() / 3);
   d.coefficients = o.coefficients.data();
   d.eps = o.eps;
+  d.half_intermediates = o.half_intermediates;
   ctx.make_current();
   WorkspaceLease ws = ctx.workspace(std::max<size_t>(blb200_newton_schulz_workspace_bytes(&d), 256));
   detail::status_check(blb200_newton_schulz(&d, ws.data(), ws.size(), ctx.native_stream()));

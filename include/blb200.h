@@ -375,7 +375,9 @@ int blb200_gemm_i8(const blb200_gemm_i8_desc* desc, void* cuda_stream);
  *     X <- G / (||G||_F + eps);   steps times:  S = X X^T,  X <- (a I + b S + c S^2) X      (rows <= cols;
  * X^T X from the right otherwise), and writes the last X to y (y may be x itself, same ld and stride).
  * coefficients: (a, b, c) once (coefficient_sets 1) or one triple per step (coefficient_sets == steps).
- * float and float16 keep every intermediate matrix as a pair of float16 matrices (float accuracy), bfloat16 as one.
+ * Every intermediate matrix is kept as a pair of float16 matrices (22 bits and a sign, float accuracy), sums in float; y is
+ * rounded once.  half_intermediates = 1 (bfloat16 only, else BLB200_E_UNSUPPORTED; 0 otherwise) keeps one float16 matrix of
+ * each instead: large calls take 0.3 of the time, and the error grows from 1.65e-3 of the result (y's rounding) to 1.9 .. 2.2e-3.
  * From the coefficients follows a bound on X's largest singular value at each step; coefficients under
  * which it passes 64, or an entry of b S + c S^2 may pass 16384, are refused with BLB200_E_TOO_LARGE.
  * steps 1 .. 64, eps >= 0, batch <= 65535.  An item that holds a NaN or an infinity comes out as NaN.
@@ -387,6 +389,7 @@ typedef struct blb200_newton_schulz_desc {
   int64_t ldx, ldy, stride_x, stride_y; /* elements */
   int32_t ftype;                        /* blb200_ftype of x and y */
   int32_t steps, coefficient_sets;
+  int32_t half_intermediates;           /* 0 or 1 */
   const double* coefficients;           /* host memory */
   double eps;
 } blb200_newton_schulz_desc;
