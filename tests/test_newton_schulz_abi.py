@@ -28,7 +28,7 @@ def test_half_intermediates_is_a_flag_for_bfloat16(lib, ftype, flag, status):
 
 def test_half_intermediates_need_half_the_scratch(lib):
     import batchlas_b200 as bl
-    x = torch.zeros(3, 1000, 2000, dtype=torch.bfloat16)
+    x = torch.zeros(3, 1024, 2048, dtype=torch.bfloat16)
     pairs, halves = bl.newton_schulz_workspace_bytes(x), bl.newton_schulz_workspace_bytes(x, half_intermediates=True)
-    matrices = 3 * 2 * (2 * 1000 * 2000 + 2 * 1000 * 1000)          # bytes of X twice, S and B in one half each
+    matrices = 3 * 2 * (2 * 1024 * 2048 + 2 * 1024 * 1024)          # bytes of X twice, S and B in one half each
     assert pairs - halves == matrices
