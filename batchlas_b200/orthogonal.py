@@ -8,7 +8,7 @@ import ctypes
 import torch
 
 from ._lib import NewtonSchulzDesc, load
-from .quantized import FTYPE_CODES, _launch, _matrix, _same_device
+from .quantized import FTYPE_CODES, _empty, _launch, _matrix, _same_device
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
 
@@ -43,18 +43,14 @@ def newton_schulz(X, Y=None, steps=5, coefficients=QUINTIC, eps=1e-7, *, half_in
     matrix of each: large calls take 0.3 of the time, and the error grows from 1.65e-3 of the result (rounding Y) to 1.9 to
     2.2e-3.  The scratch comes from torch's caching allocator unless `workspace` (a CUDA uint8 tensor, 256-byte aligned, of at
     least :func:`newton_schulz_workspace_bytes` bytes) is given.  Asynchronous."""
-    if Y is None:
-        Y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
     index = X.get_device()
-    _same_device("batchlas_b200.newton_schulz", index, Y)
+    _same_device("batchlas_b200.newton_schulz", index, *(() if Y is None else (Y,)))
+    if Y is None:
+        Y = _empty(X.shape, X.dtype, X.device, stream)
     d = _desc(X, Y, steps, coefficients, eps, half_intermediates)
     need = int(load().blb200_newton_schulz_workspace_bytes(d))
     if workspace is None:
-        if stream is None:
-            workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=X.device)
-        else:  # the scratch belongs to the stream that uses it
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, X.device) if stream else torch.cuda.default_stream(X.device)):
-                workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=X.device)
+        workspace = _empty((max(need, 256),), torch.uint8, X.device, stream, returned=False)
     elif workspace.get_device() != index or workspace.dtype is not torch.uint8 or workspace.numel() < need \
             or not workspace.is_contiguous() or workspace.data_ptr() % 256:
         raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {X.device}, 256-byte aligned")

@@ -43,6 +43,22 @@ def _launch(index, stream, fn, desc):
         check(status)
 
 
+def _empty(shape, dtype, device, stream, returned=True):
+    """Memory that a call on `stream` (None: the current one) is the first to write.  It comes from that stream's pool: a block of
+    the current stream's may still be read by what is queued there.  The caller goes on to use what is `returned` on the
+    current stream, so the allocator waits for both streams before it hands the block out again."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    current = torch.cuda.current_stream(device)
+    if current.cuda_stream == stream:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if returned:
+        t.record_stream(current)
+    return t
+
+
 def _matrix(t):
     """(batch, cols, rows, ld, stride) of a column-major tensor."""
     st = t.stride()
@@ -85,14 +101,16 @@ def _scales(where, s, batch, size, shared=True):
 
 def quantize_i8(X, Q=None, scale=None, stream=None):
     """Quantises every column of X: ``scale = max|x| * float32(1 / 127)``, ``Q = round(x / scale)``, halves to
-    even.  Q (int8, the
-    shape of X) and scale (float32, one per column) are made when they are not given; returns both.  Asynchronous."""
-    if Q is None:
-        Q = torch.empty(X.shape, dtype=torch.int8, device=X.device)
-    if scale is None:
-        scale = torch.empty(X.shape[:-1], dtype=torch.float32, device=X.device)
+    even.  Q (int8, the shape of X) and scale (float32, one per column) are made when they are not given; returns both.
+    Asynchronous."""
     index = X.get_device()
-    if index < 0 or Q.get_device() != index or scale.get_device() != index:
+    if index < 0:
+        _same_device("batchlas_b200.quantize_i8", index)
+    if Q is None:
+        Q = _empty(X.shape, torch.int8, X.device, stream)
+    if scale is None:
+        scale = _empty(X.shape[:-1], torch.float32, X.device, stream)
+    if Q.get_device() != index or scale.get_device() != index:
         _same_device("batchlas_b200.quantize_i8", index, Q, scale)
     ftype = FTYPE_CODES.get(X.dtype)
     if ftype is None:
