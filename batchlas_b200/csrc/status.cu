@@ -5,8 +5,11 @@
 
 namespace blb200 {
 int small_device_status(int* out);
+int small_device_status_clear();
 int gemv_ring_device_status(int* out);
+int gemv_ring_device_status_clear();
 int small_ring_device_status(int* out);
+int small_ring_device_status_clear();
 int dmma_tma_device_status(int* out);
 int dmma_tma_device_status_clear();
 int sgemm_tma_device_status(int* out);
@@ -17,11 +20,25 @@ int newton_schulz_device_status(int* out);
 int newton_schulz_device_status_clear();
 int newton_schulz_small_device_status(int* out);
 int newton_schulz_small_device_status_clear();
-int small_device_status_clear();
-int gemv_ring_device_status_clear();
-int small_ring_device_status_clear();
 
 namespace {
+// The status words of the library, this unit's own last: what the status call reads and the reset clears.
+struct StatusWord {
+  int (*read)(int* out);
+  int (*clear)();
+};
+constexpr StatusWord kStatusWords[] = {
+    {small_device_status, small_device_status_clear},
+    {gemv_ring_device_status, gemv_ring_device_status_clear},
+    {small_ring_device_status, small_ring_device_status_clear},
+    {dmma_tma_device_status, dmma_tma_device_status_clear},
+    {sgemm_tma_device_status, sgemm_tma_device_status_clear},
+    {gemm_i8_device_status, gemm_i8_device_status_clear},
+    {newton_schulz_device_status, newton_schulz_device_status_clear},
+    {newton_schulz_small_device_status, newton_schulz_small_device_status_clear},
+    {read_device_status_word, clear_device_status_word},
+};
+
 // One warp waits on a barrier that nothing ever arrives on.  The wait is the ring kernels' own
 // mbar_wait with a short poll limit: it gives up, records its code and the kernel returns
 // normally — no copy is in flight, nothing else shares the barrier, the context stays usable.
@@ -47,54 +64,21 @@ extern "C" int blb200_device_status(int* out) {
   *out = 0;
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return (int)e;
-  int word = 0;
-  int rc = blb200::small_device_status(&word);
-  if (rc != 0) return rc;
-  if (word == 0) {
-    rc = blb200::gemv_ring_device_status(&word);
-    if (rc != 0) return rc;
+  for (const auto& w : blb200::kStatusWords) {
+    const int rc = w.read(out);
+    if (rc != 0 || *out != 0) return rc;
   }
-  if (word == 0) {
-    rc = blb200::small_ring_device_status(&word);
-    if (rc != 0) return rc;
-  }
-  if (word == 0) {
-    rc = blb200::dmma_tma_device_status(&word);
-    if (rc != 0) return rc;
-  }
-  if (word == 0) {
-    rc = blb200::sgemm_tma_device_status(&word);
-    if (rc != 0) return rc;
-  }
-  if (word == 0) {
-    rc = blb200::gemm_i8_device_status(&word);
-    if (rc != 0) return rc;
-  }
-  if (word == 0) {
-    rc = blb200::newton_schulz_device_status(&word);
-    if (rc != 0) return rc;
-  }
-  if (word == 0) {
-    rc = blb200::newton_schulz_small_device_status(&word);
-    if (rc != 0) return rc;
-  }
-  if (word == 0) {
-    rc = blb200::read_device_status_word(&word);
-    if (rc != 0) return rc;
-  }
-  *out = word;
   return BLB200_OK;
 }
 
 extern "C" int blb200_device_status_reset(void) {
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return (int)e;
-  int rc = blb200::small_device_status_clear();
-  if (rc == 0) rc = blb200::gemv_ring_device_status_clear();
-  if (rc == 0) rc = blb200::small_ring_device_status_clear();
-  if (rc == 0) rc = blb200::dmma_tma_device_status_clear();
-  if (rc == 0) rc = blb200::sgemm_tma_device_status_clear();
-  if (rc == 0) rc = blb200::clear_device_status_word();
+  int rc = 0;
+  for (const auto& w : blb200::kStatusWords) {
+    const int e_word = w.clear();
+    if (rc == 0) rc = e_word;
+  }
   return rc;
 }
 
