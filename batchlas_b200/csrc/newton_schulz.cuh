@@ -22,16 +22,21 @@ struct Matrices {
 __host__ __device__ inline double polynomial_bound(const double* q, double top) {
   auto value = [&](double s) { return fabs(s * (q[0] + s * s * (q[1] + s * s * q[2]))); };
   double best = value(top);
-  // critical points: a + 3 b t + 5 c t^2 = 0 with t = s^2
-  const double A = 5 * q[2], B = 3 * q[1], C = q[0], disc = B * B - 4 * A * C;
-  if (A == 0) {
-    if (B != 0 && -C / B > 0 && -C / B < top * top) best = fmax(best, value(sqrt(-C / B)));
-  } else if (disc >= 0) {
-    const double r = sqrt(disc);
-    for (int i = 0; i < 2; ++i) {
-      const double t = (-B + (i ? -r : r)) / (2 * A);
-      if (t > 0 && t < top * top) best = fmax(best, value(sqrt(t)));
-    }
+  // Critical points: C + B t + A t^2 = 0 with t = (s / top)^2, its coefficients divided by the largest so that no square
+  // leaves double's range.  w adds numbers of one sign, so neither root is lost to cancellation where A or C is next to zero.
+  const double s2 = top * top;
+  double A = q[2] * s2 * s2 * 5, B = q[1] * s2 * 3, C = q[0];
+  const double size = fmax(fabs(A), fmax(fabs(B), fabs(C)));
+  if (!(size > 0)) return best;
+  A /= size;
+  B /= size;
+  C /= size;
+  const double disc = B * B - 4 * A * C;
+  if (disc >= 0) {
+    const double w = -0.5 * (B + copysign(sqrt(disc), B));
+    const double roots[2] = {w != 0 ? C / w : 0.0, A != 0 ? w / A : 0.0};
+    for (double t : roots)
+      if (t > 0 && t < 1) best = fmax(best, value(top * sqrt(t)));
   }
   return best;
 }

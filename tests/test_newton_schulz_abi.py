@@ -32,3 +32,24 @@ def test_half_intermediates_need_half_the_scratch(lib):
     pairs, halves = bl.newton_schulz_workspace_bytes(x), bl.newton_schulz_workspace_bytes(x, half_intermediates=True)
     matrices = 3 * 2 * (2 * 1024 * 2048 + 2 * 1024 * 1024)          # bytes of X twice, S and B in one half each
     assert pairs - halves == matrices
+
+
+# |a s + b s^3 + c s^5| over 0 <= s <= 1 has its maximum inside: 0.3849 a for b = -a, 0.535 a for c = -a.  With one of the coefficients
+# next to zero it still has.
+@pytest.mark.parametrize("tiny", [0.0, 1e-20, -1e-20, 1e-17, -1e-17, 1e-13, -1e-13, 1e-300])
+def test_bound_with_a_coefficient_next_to_zero(lib, tiny):
+    status = lambda *q: lib.blb200_newton_schulz(desc(q), None, 0, None)  # noqa: E731
+    assert status(200.0, -200.0, tiny) == _lib.E_TOO_LARGE        # 76.98
+    assert status(150.0, -150.0, tiny) == _lib.E_NULL             # 57.7, accepted (and then no workspace)
+    assert status(150.0, tiny, -150.0) == _lib.E_TOO_LARGE        # 80.2
+    assert status(100.0, tiny, -100.0) == _lib.E_NULL             # 53.5
+    assert status(tiny, 200.0, -200.0) == _lib.E_NULL             # 200 (s^3 - s^5): 37.2
+    assert status(tiny, 400.0, -400.0) == _lib.E_TOO_LARGE        # 74.4
+
+
+@pytest.mark.parametrize("small", [0.5, 0.1, 0.02])
+def test_bound_of_small_matrices_with_large_coefficients(lib, small):
+    """s of a second step goes up to 1.01 small; in u = s / small its polynomial is 200 (u - u^3), then 150 (u - u^3)."""
+    second = lambda a: lib.blb200_newton_schulz(desc((small, 0.0, 0.0, a / small, -a / small / small / small, 1e-20)), None, 0, None)  # noqa: E731
+    assert second(200.0) == _lib.E_TOO_LARGE
+    assert second(150.0) == _lib.E_NULL

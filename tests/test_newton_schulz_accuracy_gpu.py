@@ -99,6 +99,26 @@ def test_float_accuracy_until_the_result_is_rounded(bl, kind, batch, cols, rows)
     check(bl.newton_schulz(g.cuda()), g, kind)
 
 
+@pytest.mark.parametrize("c", [1e-20, -1e-17, 1e-13])
+@pytest.mark.parametrize("cols,rows", [(96, 80), (200, 300)])
+def test_a_coefficient_next_to_zero(bl, cols, rows, c):
+    """A step up to 1.71 before the cubic one, whose largest value then lies inside the interval."""
+    g = torch.eye(max(cols, rows))[:cols, :rows].repeat(2, 1, 1) * torch.tensor([1.0, 3e-4])[:, None, None]
+    g[1, 0, 0] = 1.0                                    # one singular value near 1, the others small
+    y = bl.newton_schulz(g.cuda(), steps=3, coefficients=[(1.7149, 0.0, 0.0), (1.5, -0.5, c), (1.5, -0.5, c)])
+    x = g.double().cuda() / (g.double().flatten(1).norm(dim=1)[:, None, None].cuda() + 1e-7)
+    d = torch.diagonal(x, dim1=1, dim2=2)
+    d = 1.7149 * d
+    for _ in range(2):
+        d = 1.5 * d - 0.5 * d ** 3 + c * d ** 5
+    got = torch.diagonal(y, dim1=1, dim2=2).double()
+    # Each stored value is off by at most e of itself (a pair, and a product of sixteen additions, the diagonal having one term).
+    # X after the first step: 2 stores of up to 1.7149; the second step's slope there is 1.5 - 1.5 * 1.7149^2 = -2.92, its two terms
+    # come to 2.57 and 2.52, from 3 stores; the third step's slope is at most 1.5, its terms below 1 from 3 stores; Y is rounded.
+    e = 2.0 ** -22 + 17 * 2.0 ** -23
+    assert float((got - d).abs().max()) <= e * (2 * 1.7149 * 2.92 * 1.5 + 3 * 5.09 * 1.5 + 3) + 2.0 ** -24 * float(d.abs().max())
+
+
 @pytest.mark.parametrize("batch,cols,rows", [(3, 128, 128), (1, 128, 4000), (2, 300, 260), (1, 1500, 1333)])
 def test_half_intermediates(bl, batch, cols, rows):
     """One float16 matrix each, and sums that stay in tensor memory for as long as they are."""
