@@ -22,8 +22,9 @@ FTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 # These calls are short, so their host side is kept short too: plain integers instead of views, no device guard or stream
-# object where the current ones are the right ones.
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# object where the current ones are the right ones (builds of torch without the short way to the current stream, CPU builds
+# among them, take the public one).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _same_device(where, index, *ts):
