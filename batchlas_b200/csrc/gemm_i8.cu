@@ -246,7 +246,9 @@ struct I8Epilogue::Tile {
 
 // Estimated time of one way to cut C into tiles, in SM cycles: rounds of tiles, each as long as the slower of its MMAs
 // (8192 products per cycle) and of its fetches (about 50 bytes per cycle and SM from L2), and about 2500 cycles for filling the ring
-// and the epilogue; splitting k costs an exchange of about 1500.
+// and the epilogue; splitting k costs an exchange of about 1500.  With plain loads a block of k takes 1.25 us at 64 columns and 1.5
+// at 128, a tile's start and end 1.7 and 3, a split 2.7 more (fitted to all choices at twenty sizes, 1.9 GHz): that picks the
+// fastest of the seven, or one within 2 % of it, from 17 x 4096 x 129 to 8192 x 1001 x 8191, but for 20 x 100 x 200 (12.9 us, 11.6 split).
 struct TileChoice {
   int group, bn, split;
   double time;
@@ -257,8 +259,10 @@ double tile_time(const GemmI8Params& p) {
   const long long units = umma_capacity<UmmaConfig<true, false, false, GROUP, BN, 1, SPLIT, PLAIN>, I8Epilogue>();
   const long long tiles = (long long)((p.m + kBM - 1) / kBM) * ((p.n + BN - 1) / BN) * p.batch;
   if (SPLIT > 1 && tiles > units) return 1e300;
-  const double blocks = (double)((p.k + 127) / 128), per = std::max(2.0 * BN, (16384.0 + 128.0 * BN / GROUP) / 50.0);
-  return (double)((tiles + units - 1) / units) * (ceil(blocks / SPLIT) * per + 2500.0) + (SPLIT > 1 ? 1500.0 : 0.0);
+  const double blocks = (double)((p.k + 127) / 128);
+  const double per = PLAIN ? 1900.0 + 7.5 * BN : std::max(2.0 * BN, (16384.0 + 128.0 * BN / GROUP) / 50.0);
+  const double tile = PLAIN ? 700.0 + 40.0 * BN : 2500.0, exchange = SPLIT == 1 ? 0.0 : PLAIN ? 5100.0 : 1500.0;
+  return (double)((tiles + units - 1) / units) * (ceil(blocks / SPLIT) * per + tile) + exchange;
 }
 template <bool PLAIN>
 TileChoice choose_tiles(const GemmI8Params& p) {
