@@ -244,7 +244,7 @@ int launch_quantize(const QuantizeParams& p, cudaStream_t stream) {
   constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1;
   const long long total = (long long)p.cols * p.batch, units = p.k / V;
   // units per thread: one where there are few columns to fill the machine with, else enough to make a thread worth its start
-  const bool few = total * ((units + 3) / 4) < 148ll * 1024;
+  const bool few = total * ((units + 3) / 4) < device_info().sm_count * 1024ll;
   const int per = few && units <= 1024 ? 1 : WIDE ? (units < 256 ? 4 : 8) : (units < 256 ? 4 : 16);
   const long long threads = (units + per - 1) / per;
   if (threads > 1024) {
