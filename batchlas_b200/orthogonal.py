@@ -4,6 +4,7 @@ row-major matrix can be passed as it is."""
 from __future__ import annotations
 
 import ctypes
+import numbers
 
 import torch
 
@@ -21,7 +22,7 @@ def _desc(X, Y, steps, coefficients, eps, half_intermediates):
     if (batch, cols, rows) != (y_batch, y_cols, y_rows):
         raise RuntimeError("NEWTON_SCHULZ: incompatible matrix dimensions")
     sets = list(coefficients)
-    if len(sets) == 3 and isinstance(sets[0], (int, float)):
+    if len(sets) == 3 and isinstance(sets[0], numbers.Real):
         sets = [sets]
     if len(sets) not in (1, steps) or any(len(s) != 3 for s in sets):
         raise ValueError("newton_schulz: coefficients are one triple (a, b, c), or one for each step")

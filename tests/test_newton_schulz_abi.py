@@ -53,3 +53,17 @@ def test_bound_of_small_matrices_with_large_coefficients(lib, small):
     second = lambda a: lib.blb200_newton_schulz(desc((small, 0.0, 0.0, a / small, -a / small / small / small, 1e-20)), None, 0, None)  # noqa: E731
     assert second(200.0) == _lib.E_TOO_LARGE
     assert second(150.0) == _lib.E_NULL
+
+
+@pytest.mark.parametrize("coefficients", [QUINTIC, list(QUINTIC), (3, -4, 2)], ids=str)
+@pytest.mark.parametrize("form", ["as is", "float32 array", "one per step"])
+def test_forms_of_the_coefficients(lib, coefficients, form):
+    import numpy as np
+
+    from batchlas_b200.orthogonal import _desc
+    given = {"as is": coefficients, "float32 array": np.array(coefficients, np.float32), "one per step": [coefficients] * 4}[form]
+    x = torch.zeros(2, 3, 4)
+    d = _desc(x, x, 4, given, 1e-7, False)
+    sets = 4 if form == "one per step" else 1
+    want = [float(np.float32(v)) if form == "float32 array" else float(v) for v in coefficients] * sets
+    assert d.coefficient_sets == sets and d.coefficients[:3 * sets] == want
