@@ -119,15 +119,23 @@ def test_a_coefficient_next_to_zero(bl, cols, rows, c):
     assert float((got - d).abs().max()) <= e * (2 * 1.7149 * 2.92 * 1.5 + 3 * 5.09 * 1.5 + 3) + 2.0 ** -24 * float(d.abs().max())
 
 
-@pytest.mark.parametrize("batch,cols,rows", [(3, 128, 128), (1, 128, 4000), (2, 300, 260), (1, 1500, 1333)])
+@pytest.mark.parametrize("batch,cols,rows", [(3, 128, 128), (1, 128, 4000), (2, 300, 260), (1, 1500, 1333), (300, 50, 60), (2, 128, 250), (1, 64, 1000),
+                                             (1, 1000, 64), (1, 385, 256), (2, 520, 513), (1, 3000, 128), (9, 515, 1030), (2, 2111, 1700)])
 def test_half_intermediates(bl, batch, cols, rows):
     """One float16 matrix each, and sums that stay in tensor memory for as long as they are."""
     g = update_like(batch, cols, rows, cols + rows, "bf16")
     y = bl.newton_schulz(g.cuda(), half_intermediates=True)
-    check(y, g, "bf16", store=HALF, additions=max(cols, rows) // 16)
+    check(y, g, "bf16", store=HALF, additions=max(cols, rows) // 16 + 1)
     assert not torch.equal(y, bl.newton_schulz(g.cuda()))
     space = torch.empty(bl.newton_schulz_workspace_bytes(g, half_intermediates=True), dtype=torch.uint8, device="cuda")
     assert torch.equal(y, bl.newton_schulz(g.cuda(), half_intermediates=True, workspace=space))
+    padded = torch.full((batch, cols, rows + 3), 7.0, dtype=torch.bfloat16, device="cuda")
+    view = padded[:, :, 1:rows + 1]
+    view.copy_(g)
+    bl.newton_schulz(view, view, half_intermediates=True)
+    assert torch.equal(view, y)
+    view.fill_(7.0)
+    assert bool((padded == 7.0).all())
 
 
 def test_half_intermediates_are_for_bfloat16_alone(bl):
