@@ -16,8 +16,9 @@
 // exchange.  A wait that runs out lets the CTA go through the remaining barriers without products.
 //
 // Bound by latency: a product, its completion, the epilogue's pass over tensor and shared memory and two barriers of the CTA take
-// about 1.5 us (5 us for a step of 128 x 128 bfloat16, 8 to 11 with a cluster's exchange), against 6 for a launch of its own:
-// 64 of 128 x 128 bfloat16 34 us (98 as products over all items), 128 x 2048 71 us (about 115).
+// about 3.3 us as pairs (10 us for a step of 128 x 128, 13 with 256 columns, 20 with a cluster's exchange) and 2.3 in single
+// halves: 64 of 128 x 128 take 53 us (35 in single halves, where they took 98 as products over all items), 14 of 128 x 2048
+// 117 us (78); fifteen as products 175 (122).
 #include "newton_schulz.cuh"
 #include "tcgen05.cuh"
 
@@ -399,8 +400,9 @@ int launch_by_size(const Matrices& g, const Matrices& y, const Plan& plan, cudaS
 }  // namespace
 
 // The shorter side in one tile and the longer one in the shared memory of a cluster.  Batches whose clusters do not all run at
-// once (about 14 of eight CTAs do, one CTA per SM) are as fast or faster as products over all items: 14 matrices of 128 x 4096 bfloat16
-// take 92 us here, and fifteen 165 as products, where sixteen would take 173 here.
+// once (about 14 of eight CTAs do, one CTA per SM) are as fast or faster as products over all items: 14 matrices of 128 x 4096 in
+// single halves take 101 us here, and fifteen 165 as products, where two rounds here take 173.  The 112 CTAs are a constant, not
+// asked of the device, because the size of the scratch follows from this and must not depend on the device that is current.
 bool newton_schulz_small_supported(int rows, int cols, int batch, int planes) {
   const int p = rows < cols ? rows : cols, q = rows < cols ? cols : rows;
   if (p > 128 || q > (planes == 1 ? 4096 : 2048)) return false;

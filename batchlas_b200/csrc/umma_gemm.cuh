@@ -20,11 +20,12 @@
 // distributed shared memory (the idle stages), each CTA adding up, in rank order, what it stores.  For calls whose
 // tiles would leave most SMs without work.
 // PLAIN: the operands are not on 16-byte boundaries, so the eight epilogue warps fetch the stages themselves, as aligned words
-// shifted together and written where the swizzle puts them (777 x 4099 x 1003 with its quantisation 37 us; a row at a time, one word
+// shifted together and written where the swizzle puts them (777 x 4099 x 1003 with its quantisation 32 us; a row at a time, one word
 // per lane and the neighbour's by a shuffle, measured 52).
 //
-// Measured: 8192^3 8-bit 380 us = 2.9 POP/s, where the MMAs alone, without fetches and stores, take 345 and the fetches alone 215;
-// half precision, 4096 x 4096 x 16384, 411 us = 1.34 PFLOP/s under the power limit.  The MMAs are what bounds large
+// Measured: 8192^3 8-bit 380 us = 2.9 POP/s in a burst (within a full call about 440, at the clock the power limit leaves), where the MMAs alone, without fetches and stores, take 345 and the fetches alone 215;
+// half precision, 4096 x 4096 x 16384, 411 us = 1.34 PFLOP/s under the power limit; pairs of halves, 8192 x 4096 x 4096, 726 us,
+// 1.14 PFLOP/s of three MMAs per product.  The MMAs are what bounds large
 // products; small ones are bounded by the 5 to 7 us between the start of one product and the start of the next that
 // needs it (first fetch 1 to 2 us, k blocks 0.3 us each with six in flight, epilogue 1, storing and the next start 2).
 //

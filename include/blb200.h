@@ -333,7 +333,8 @@ typedef enum { BLB200_F32 = 0, BLB200_F16 = 1, BLB200_BF16 = 2 } blb200_ftype;
 
 /* Quantises every column of a batch of k x cols matrices:
  *     scale_j = fl32(max_i |x_ij| * fl32(1 / 127)),   q_ij = min(127, max(-127, rne(fl32(x_ij / scale_j))))
- * with fl32 the rounding to float and rne the nearest integer, halves to the even one.  A column
+ * with fl32 the rounding to float and rne the nearest integer, halves to the even one.  (1 / 127 is rounded as well, so for one
+ * column in twenty scale_j is the float next to max / 127.)  A column
  * whose scale is 0 gets zeros (so an empty or all-zero column is exact); a column that holds a NaN or
  * an infinity gets that as its scale, and zeros, so a product made with it is NaN there.
  * scale: float, element j of item b at scale[b*stride_scale + j].  x, q and scale must not overlap.
