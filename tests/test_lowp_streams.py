@@ -101,3 +101,30 @@ def test_a_block_that_queued_work_still_reads_is_not_written(lib, call):
     assert all(bool((c == 0x5a).all()) for c in copies)
     assert all(torch.equal(g, w) for g, w in zip(got, want))
     assert bl.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_outputs_made_on_a_side_stream_of_a_capture(lib):
+    import batchlas_b200 as bl
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(40, 512, generator=gen).cuda()
+    side = torch.cuda.Stream()
+    bl.quantize_i8(x), bl.newton_schulz(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        q, s = bl.quantize_i8(x, stream=side.cuda_stream)
+        y = bl.newton_schulz(x, stream=side.cuda_stream)
+        for _ in range(3):                       # dropped at once
+            bl.quantize_i8(x, stream=side.cuda_stream), bl.newton_schulz(x, stream=side.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+        values = q * s[:, None]
+    for _ in range(3):
+        x.copy_(torch.randn(40, 512, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        want_q, want_s = bl.quantize_i8(x)
+        assert torch.equal(q, want_q) and torch.equal(s, want_s) and torch.equal(values, want_q * want_s[:, None])
+        assert torch.equal(y, bl.newton_schulz(x))
+    assert bl.device_status() == 0
